@@ -65,6 +65,45 @@ internal static unsafe partial class NnHipNative
         internal int XHeadWidth; internal int XHeadGroup; internal uint PostOp; internal uint Reserved;
     }
 
+    internal const int KvBlockTokens = 64, LogProbsMaxTop = 64;
+    internal const uint RotaryHalves = 0, RotaryPairs = 1;
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal struct RowsDesc
+    {
+        internal nint Data; internal long TokenStride; internal long SequenceStride;
+    }
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal struct KvCacheDesc
+    {
+        internal uint StructSize; internal int Sequences; internal int KvHeads; internal int HeadWidth; internal int Capacity;
+        internal uint Reserved; internal nint Data; internal nint Lengths;
+    }
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal struct KvStoreDesc
+    {
+        internal uint StructSize; internal int Tokens; internal nint Counts;
+        internal RowsDesc K; internal RowsDesc V; internal RowsDesc Q; internal RowsDesc QOut;
+        internal nint InvFreq; internal int RotaryWidth; internal uint RotaryStyle; internal int Heads; internal uint Reserved;
+    }
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal struct AttentionDesc
+    {
+        internal uint StructSize; internal int Tokens; internal nint Counts; internal RowsDesc Q; internal RowsDesc Out;
+        internal int Heads; internal int Window; internal int Sinks; internal float Scale;
+    }
+
+    [StructLayout(LayoutKind.Sequential)]
+    internal struct LogProbsDesc
+    {
+        internal uint StructSize; internal int Rows; internal int Vocabulary; internal int Top; internal long RowStride;
+        internal nint Logits; internal nint Targets; internal nint LogProbs; internal nint Entropy; internal nint TopIds;
+        internal nint TopLogProbs;
+    }
+
     [LibraryImport(Library)] internal static partial uint nnhip_abi_version();
     [LibraryImport(Library)] internal static partial int nnhip_last_error(out ErrorInfo info, nuint size);
     [LibraryImport(Library)] internal static partial int nnhip_last_error_message(byte* buffer, int capacity);
@@ -106,6 +145,12 @@ internal static unsafe partial class NnHipNative
     [LibraryImport(Library)] internal static partial int nnhip_first_token_attention(nint lane, nint v, nint output, int heads, int kvHeads, int headWidth);
     [LibraryImport(Library)] internal static partial int nnhip_lora_a(nint lane, nint x, nint a, nint z, int rows, int width, int rank);
     [LibraryImport(Library)] internal static partial int nnhip_lora_b(nint lane, nint z, nint b, nint y, int rows, int output, int rank, float scale);
+    [LibraryImport(Library)] internal static partial int nnhip_kv_cache_bytes(int sequences, int kvHeads, int headWidth, int capacity, out ulong bytes);
+    [LibraryImport(Library)] internal static partial int nnhip_kv_cache_store(nint lane, KvCacheDesc* cache, KvStoreDesc* desc);
+    [LibraryImport(Library)] internal static partial int nnhip_kv_cache_advance(nint lane, KvCacheDesc* cache, int tokens, nint counts);
+    [LibraryImport(Library)] internal static partial int nnhip_kv_cache_read(nint lane, KvCacheDesc* cache, nint first, int tokens, RowsDesc* kOut, RowsDesc* vOut);
+    [LibraryImport(Library)] internal static partial int nnhip_cached_attention(nint lane, KvCacheDesc* cache, AttentionDesc* desc);
+    [LibraryImport(Library)] internal static partial int nnhip_token_log_probs(nint lane, LogProbsDesc* desc);
     [LibraryImport(Library)] internal static partial int nnhip_event_create(nint lane, out nint evt);
     [LibraryImport(Library)] internal static partial int nnhip_event_destroy(nint lane, nint evt);
     [LibraryImport(Library)] internal static partial int nnhip_event_record(nint lane, nint evt);

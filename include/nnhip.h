@@ -68,7 +68,7 @@ enum {
     NNHIP_OP_UPLOAD, NNHIP_OP_DOWNLOAD, NNHIP_OP_COPY, NNHIP_OP_SYNCHRONIZE, NNHIP_OP_DEQUANTIZE,
     NNHIP_OP_MATVEC, NNHIP_OP_MATVEC_BATCH, NNHIP_OP_MATMUL_BF16, NNHIP_OP_EVENT, NNHIP_OP_GRAPH,
     NNHIP_OP_DEVICE_QUERY, NNHIP_OP_FILL, NNHIP_OP_RMS_NORM, NNHIP_OP_SILU_MULTIPLY, NNHIP_OP_ADD_IN_PLACE,
-    NNHIP_OP_MATVEC_FUSED, NNHIP_OP_LORA, NNHIP_OP_ATTENTION, NNHIP_OP_MATMUL
+    NNHIP_OP_MATVEC_FUSED, NNHIP_OP_LORA, NNHIP_OP_ATTENTION, NNHIP_OP_MATMUL, NNHIP_OP_KV_CACHE, NNHIP_OP_LOG_PROBS
 };
 
 /* Same field order as the reference's NativeErrorInfo (CudaNativeGateway.cs:1360-1371). */
@@ -441,6 +441,130 @@ NNHIP_API int nnhip_first_token_attention(void* lane, const float* v, float* out
 NNHIP_API int nnhip_lora_a(void* lane, const float* x, const float* a, float* z, int rows, int width, int rank);
 NNHIP_API int nnhip_lora_b(void* lane, const float* z, const float* b, float* y, int rows, int output, int rank,
                            float scale);
+
+/* --- 8-bit key/value cache, attention over it, token log probabilities ---------------------------------------- */
+
+/* The cache of one layer: keys and values of `sequences` sequences of up to `capacity` tokens, `kv_heads` heads of
+ * `head_width` (1 - 256) values, in 8 bits with one scale for each block: NNHIP_KV_BLOCK_TOKENS consecutive tokens (token t
+ * belongs to block t / NNHIP_KV_BLOCK_TOKENS) of one head, keys and values apart.  For a block whose tokens so far hold the
+ * values x, over all head_width components:
+ *     scale = max |x| / 127 (rounded to FP32 once),  code = rint(x / scale) (the exact quotient, half to even),  |code| <= 127
+ * and the cache stands for the values scale * code.  An all-zero block has scale 0.  A NaN or an infinity in a block makes
+ * its scale NaN.  The cache after n tokens does not depend on how they were split over nnhip_kv_cache_store calls: the FP32
+ * values of the block that is not full yet are kept beside it and quantised again when its largest magnitude grows.
+ * `data` holds nnhip_kv_cache_bytes bytes of device memory on a 16-byte boundary; its contents need no initialisation and
+ * their order is the library's own.  `lengths` [sequences] is device memory: the tokens each sequence holds BEFORE the step
+ * at hand.  The entries below read it when they run, so one captured graph serves every length; nnhip_kv_cache_advance adds
+ * the step's tokens after its last layer.  Layers of one model share a lengths array.  A sequence whose length is negative,
+ * or whose tokens of this call would pass `capacity`, is left out: nothing of it is stored, and its rows of the attention's
+ * output become NaN.  Lengths may be set back (to drop the last tokens, or start over).  Tokens that stay in a block which
+ * was not the last one stored count with their 8-bit values when that block is filled up again. */
+#define NNHIP_KV_BLOCK_TOKENS 64
+typedef struct nnhip_kv_cache {
+    uint32_t struct_size;
+    int32_t sequences;
+    int32_t kv_heads;
+    int32_t head_width;
+    int32_t capacity;           /* tokens for each sequence */
+    uint32_t reserved;          /* 0 */
+    void* data;
+    int32_t* lengths;           /* device, [sequences] */
+} nnhip_kv_cache;
+
+/* FP32 rows [sequence, token, heads * width]: element (b, i, c) is data[b * sequence_stride + i * token_stride + c].  Strides
+ * are in floats and not negative (an input may use 0 to repeat a row); the rows of an output must not overlap. */
+typedef struct nnhip_rows {
+    float* data;
+    int64_t token_stride;
+    int64_t sequence_stride;
+} nnhip_rows;
+
+/* Bytes of device memory for `data`. */
+NNHIP_API int nnhip_kv_cache_bytes(int sequences, int kv_heads, int head_width, int capacity, uint64_t* bytes);
+
+/* Stores `tokens` new tokens of every sequence (counts [sequences], device, nullable: the first counts[b] of them; values
+ * outside 0..tokens count as the nearest of the two) at positions lengths[b], lengths[b] + 1, ...  With inv_freq (device,
+ * [rotary_width / 2]) keys are turned by rotary positions first: pair j of the first rotary_width components of every head
+ * turns by the angle position * inv_freq[j], computed in 64 bits and rounded to FP32 once.  The pairs are (j, j + rotary_width / 2) for
+ * NNHIP_ROTARY_HALVES and (2j, 2j + 1) for NNHIP_ROTARY_PAIRS.  q (nullable) holds `heads` query heads of the same tokens: they
+ * are turned the same way into q_out, which may be q itself; q needs inv_freq.  Rows behind counts[b] are neither read nor
+ * written.  lengths stays as it is.  Replaces the rotary and cache-append launches of Qwen35Gpu.AttentionStep
+ * (NNtrain.Core/Modules/Qwen35Gpu.Attention.cs:60-120).  Asynchronous. */
+enum { NNHIP_ROTARY_HALVES = 0, NNHIP_ROTARY_PAIRS = 1 };
+typedef struct nnhip_kv_store_desc {
+    uint32_t struct_size;
+    int32_t tokens;
+    const int32_t* counts;
+    nnhip_rows k;
+    nnhip_rows v;
+    nnhip_rows q;
+    nnhip_rows q_out;
+    const float* inv_freq;
+    int32_t rotary_width;       /* even, 2 .. head_width; 0 without inv_freq */
+    uint32_t rotary_style;
+    int32_t heads;              /* query heads; 0 without q */
+    uint32_t reserved;          /* 0 */
+} nnhip_kv_store_desc;
+NNHIP_API int nnhip_kv_cache_store(void* lane, const nnhip_kv_cache* cache, const nnhip_kv_store_desc* desc);
+
+/* lengths[b] += counts[b] (clamped to 0..tokens), or += tokens without counts.  A sequence that nnhip_kv_cache_store would
+ * have left out keeps its length.  Asynchronous. */
+NNHIP_API int nnhip_kv_cache_advance(void* lane, const nnhip_kv_cache* cache, int tokens, const int32_t* counts);
+
+/* FP32 values (scale * code) of tokens first[b] .. first[b] + tokens - 1 (first: device, [sequences], nullable: 0).  Tokens
+ * outside 0 .. capacity - 1 read as 0; what a token that was never stored reads as is not defined (0 behind the last token
+ * of the last block stored).  k_out.data or v_out.data may be null.  Asynchronous. */
+NNHIP_API int nnhip_kv_cache_read(void* lane, const nnhip_kv_cache* cache, const int32_t* first, int tokens,
+                                  const nnhip_rows* k_out, const nnhip_rows* v_out);
+
+/* Attention of the tokens that nnhip_kv_cache_store has just stored (same tokens, counts and lengths): query row (b, i, h)
+ * stands at position p = lengths[b] + i and sees key t of head h / (heads / kv_heads) when
+ *     t <= p  and  (window == 0  or  t > p - window  or  t < sinks),
+ *     out[b, i, h] = sum_t softmax_t(scale * q . K_t) V_t  over the keys it sees (always its own at least).
+ * Rows behind counts[b] are not written.  heads is a multiple of kv_heads; scale is finite and >= 0; out must not overlap q.
+ * FP32 in and out: queries and probabilities enter the matrix cores as two half-precision parts (22 bits of the largest
+ * component of a query row, of the largest probability times value scale), the codes are exact there, all sums and
+ * softmax statistics are FP32.  A row that sees a token of a block whose scale is NaN, or whose query holds a NaN or an
+ * infinity, is NaN; keys a row does not see have no influence on it.  Results do not depend on the other sequences of the
+ * call and are the same on every run.  Scratch memory comes from the lane's kept blocks as in nnhip_quant_matmul.  Replaces the attention core of Qwen35Gpu.AttentionStep
+ * (Qwen35Gpu.Attention.cs:60-120).  Asynchronous. */
+typedef struct nnhip_attention_desc {
+    uint32_t struct_size;
+    int32_t tokens;
+    const int32_t* counts;
+    nnhip_rows q;
+    nnhip_rows out;
+    int32_t heads;
+    int32_t window;             /* 0: no limit */
+    int32_t sinks;
+    float scale;
+} nnhip_attention_desc;
+NNHIP_API int nnhip_cached_attention(void* lane, const nnhip_kv_cache* cache, const nnhip_attention_desc* desc);
+
+/* For every row of logits [rows, vocabulary] (row_stride floats apart), with p = softmax(row):
+ *     log_probs[r] = ln p[targets[r]]                      (targets null: not computed; a target outside the vocabulary: NaN)
+ *     entropy[r]   = - sum_v p[v] ln p[v]                  (nullable)
+ *     top_ids[r, 0..top), top_log_probs[r, 0..top)         the `top` (0 - NNHIP_LOG_PROBS_MAX_TOP) largest logits, largest
+ *                                                          first, equal ones by index; top_log_probs is nullable.
+ * One pass over the logits; sums are kept in 64 bits, so that the log probability of a near-certain token and the entropy of
+ * a peaked row keep their FP32 accuracy.  A logit of -infinity has probability 0.  A row that holds a NaN or +infinity, or
+ * nothing above -infinity, has NaN log probabilities and entropy; in the order of top_ids a NaN counts as +infinity.  Deterministic.  The reference downloads the logits and works on the
+ * host (QwenGgufCommand.cs:119-157).  Asynchronous. */
+#define NNHIP_LOG_PROBS_MAX_TOP 64
+typedef struct nnhip_log_probs_desc {
+    uint32_t struct_size;
+    int32_t rows;
+    int32_t vocabulary;
+    int32_t top;
+    int64_t row_stride;
+    const float* logits;
+    const int32_t* targets;
+    float* log_probs;
+    float* entropy;
+    int32_t* top_ids;
+    float* top_log_probs;
+} nnhip_log_probs_desc;
+NNHIP_API int nnhip_token_log_probs(void* lane, const nnhip_log_probs_desc* desc);
 
 /* --- timing and replay --------------------------------------------------------------------------------------- */
 

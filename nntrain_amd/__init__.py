@@ -15,4 +15,5 @@ from .quantized_matrix import (BLOCK_BYTES, BLOCK_ELEMS, GGML_BF16, GGML_IQ2_S, 
 from .gguf import GgufReader, GgufReadLimits, GgufTensorInfo, InvalidDataError  # noqa: F401
 from .loader import GgufTensorDirectory, HipGgufLoader, NotSupportedError  # noqa: F401
 from . import qwen35_gpu  # noqa: F401
+from .kv_cache import QuantizedKvCache, Rotary, Rows  # noqa: F401
 from .decoder import DecoderDescriptor, GenerationTiming, QuantizedDecoder  # noqa: F401

@@ -8,6 +8,7 @@
 
 #include <unistd.h>
 
+#include "kv_cache_layout.h"
 #include "nnhip_internal.h"
 
 namespace nnhip {
@@ -728,6 +729,188 @@ int nnhip_first_token_attention(void* handle, const float* v, float* out, int he
         return fail(NNHIP_ERR_TOO_LARGE, NNHIP_OP_ATTENTION, lane->device, 0, "heads * head_width exceeds one launch");
     hipError_t e = launch_first_token_attention(lane, v, out, heads, kv_heads, head_width);
     if (e != hipSuccess) return hip_fail(e, NNHIP_OP_ATTENTION, lane->device, "first-token attention launch");
+    lane->counters.kernel_launches += 1;
+    return NNHIP_OK;
+}
+
+// --- 8-bit key/value cache ---------------------------------------------------------------------------------------
+
+// Checks a cache descriptor and derives its layout; `lane` is null for the size query.
+static int kv_cache_of(uint32_t op, nnhip::Lane* lane, const nnhip_kv_cache* c, nnhip::KvLayout* out)
+{
+    using namespace nnhip;
+    if (!c || c->struct_size != sizeof(nnhip_kv_cache) || c->reserved != 0)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "cache is null, has the wrong struct_size or a reserved field that is not 0");
+    if (c->sequences < 1 || c->kv_heads < 1 || c->head_width < 1 || c->capacity < 1)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "sequences, kv_heads, head_width and capacity must be positive");
+    if (c->head_width > kKvMaxWidth)
+        return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "head_width %d exceeds %d", c->head_width, kKvMaxWidth);
+    if (!c->data || !c->lengths || (reinterpret_cast<uintptr_t>(c->data) & 15u) || (reinterpret_cast<uintptr_t>(c->lengths) & 3u))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "data must be 16-byte aligned and lengths 4-byte aligned, both non-null");
+    uint64_t bytes = 0;
+    if (!kv_layout(c->sequences, c->kv_heads, c->head_width, c->capacity, out, &bytes))
+        return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "the cache is too large");
+    out->base = static_cast<uint8_t*>(c->data);
+    out->lengths = c->lengths;
+    return NNHIP_OK;
+}
+
+// Checks an operand of rows [sequences, tokens, width].  Rows of an output must not overlap.
+static int check_rows(uint32_t op, nnhip::Lane* lane, const nnhip_rows& r, int sequences, int tokens, int64_t width, bool output, const char* name)
+{
+    using namespace nnhip;
+    if (!r.data || (reinterpret_cast<uintptr_t>(r.data) & 3u))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "%s is null or not 4-byte aligned", name);
+    if (r.token_stride < 0 || r.sequence_stride < 0)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "the strides of %s must not be negative", name);
+    const __int128 t = r.token_stride, s = r.sequence_stride;
+    if ((t * (tokens - 1) + s * (sequences - 1) + width) >> 60)
+        return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "%s is too large", name);
+    const bool inner_tokens = (tokens == 1 || t >= width) && (sequences == 1 || s >= t * (tokens - 1) + width);
+    const bool inner_sequences = (sequences == 1 || s >= width) && (tokens == 1 || t >= s * (sequences - 1) + width);
+    if (output && !inner_tokens && !inner_sequences)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "the rows of %s overlap", name);
+    return NNHIP_OK;
+}
+
+int nnhip_kv_cache_bytes(int sequences, int kv_heads, int head_width, int capacity, uint64_t* bytes)
+{
+    if (!bytes || sequences < 1 || kv_heads < 1 || head_width < 1 || capacity < 1)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, NNHIP_OP_KV_CACHE, -1, 0, "sequences, kv_heads, head_width and capacity must be positive and bytes non-null");
+    KvLayout layout;
+    if (head_width > kKvMaxWidth || !kv_layout(sequences, kv_heads, head_width, capacity, &layout, bytes))
+        return fail(NNHIP_ERR_TOO_LARGE, NNHIP_OP_KV_CACHE, -1, 0, "head_width exceeds %d or the cache is too large", kKvMaxWidth);
+    return NNHIP_OK;
+}
+
+int nnhip_kv_cache_store(void* handle, const nnhip_kv_cache* cache, const nnhip_kv_store_desc* d)
+{
+    const uint32_t op = NNHIP_OP_KV_CACHE;
+    NNHIP_LANE(handle, op)
+    KvLayout layout;
+    int rc = kv_cache_of(op, lane, cache, &layout);
+    if (rc != NNHIP_OK) return rc;
+    if (!d || d->struct_size != sizeof(nnhip_kv_store_desc) || d->reserved != 0)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "descriptor is null, has the wrong struct_size or a reserved field that is not 0");
+    if (d->tokens < 1) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive");
+    if (d->inv_freq) {
+        if (d->rotary_width < 2 || d->rotary_width % 2 != 0 || d->rotary_width > layout.head_width || d->rotary_style > NNHIP_ROTARY_PAIRS)
+            return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "rotary_width must be even and within the head, rotary_style a known one");
+    } else if (d->rotary_width != 0 || d->q.data) {
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "rotary_width and q need inv_freq");
+    }
+    const int64_t kv_width = static_cast<int64_t>(layout.kv_heads) * layout.head_width;
+    rc = check_rows(op, lane, d->k, layout.sequences, d->tokens, kv_width, false, "k");
+    if (rc == NNHIP_OK) rc = check_rows(op, lane, d->v, layout.sequences, d->tokens, kv_width, false, "v");
+    if (rc != NNHIP_OK) return rc;
+    if (d->q.data) {
+        if (d->heads < 1) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "heads must be positive with q");
+        const int64_t q_width = static_cast<int64_t>(d->heads) * layout.head_width;
+        if (q_width > 0x7fffffff) return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "heads * head_width exceeds one launch");
+        rc = check_rows(op, lane, d->q, layout.sequences, d->tokens, q_width, false, "q");
+        if (rc == NNHIP_OK) rc = check_rows(op, lane, d->q_out, layout.sequences, d->tokens, q_width, true, "q_out");
+        if (rc != NNHIP_OK) return rc;
+        if (d->q.data == d->q_out.data && (d->q.token_stride != d->q_out.token_stride || d->q.sequence_stride != d->q_out.sequence_stride))
+            return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "q_out over q needs q's strides");
+    } else if (d->heads != 0 || d->q_out.data) {
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "heads and q_out need q");
+    }
+    const int64_t pairs = static_cast<int64_t>(layout.sequences) * layout.kv_heads;
+    if (pairs * 2 * (d->tokens / kKvBlock + 2) + static_cast<int64_t>(layout.sequences) * d->tokens > 0x7fffffff || kv_width > 0x3fffffff)
+        return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, heads and tokens exceed one launch");
+    const hipError_t e = launch_kv_store(lane, layout, *d);
+    if (e != hipSuccess) return hip_fail(e, op, lane->device, "cache store launch");
+    lane->counters.kernel_launches += 1;
+    return NNHIP_OK;
+}
+
+int nnhip_kv_cache_advance(void* handle, const nnhip_kv_cache* cache, int tokens, const int32_t* counts)
+{
+    const uint32_t op = NNHIP_OP_KV_CACHE;
+    NNHIP_LANE(handle, op)
+    KvLayout layout;
+    const int rc = kv_cache_of(op, lane, cache, &layout);
+    if (rc != NNHIP_OK) return rc;
+    if (tokens < 1) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive");
+    const hipError_t e = launch_kv_advance(lane, layout, tokens, counts);
+    if (e != hipSuccess) return hip_fail(e, op, lane->device, "cache advance launch");
+    lane->counters.kernel_launches += 1;
+    return NNHIP_OK;
+}
+
+int nnhip_kv_cache_read(void* handle, const nnhip_kv_cache* cache, const int32_t* first, int tokens, const nnhip_rows* k_out,
+                        const nnhip_rows* v_out)
+{
+    const uint32_t op = NNHIP_OP_KV_CACHE;
+    NNHIP_LANE(handle, op)
+    KvLayout layout;
+    int rc = kv_cache_of(op, lane, cache, &layout);
+    if (rc != NNHIP_OK) return rc;
+    if (tokens < 1) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive");
+    const nnhip_rows none{nullptr, 0, 0}, k = k_out ? *k_out : none, v = v_out ? *v_out : none;
+    const int64_t width = static_cast<int64_t>(layout.kv_heads) * layout.head_width;
+    if (!k.data && !v.data) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "k_out and v_out are both null");
+    if (k.data) rc = check_rows(op, lane, k, layout.sequences, tokens, width, true, "k_out");
+    if (rc == NNHIP_OK && v.data) rc = check_rows(op, lane, v, layout.sequences, tokens, width, true, "v_out");
+    if (rc != NNHIP_OK) return rc;
+    const int64_t pairs = static_cast<int64_t>(layout.sequences) * layout.kv_heads;
+    if (pairs * 2 * (tokens / kKvBlock + 2) > 0x7fffffff || static_cast<int64_t>(layout.sequences) * tokens > 0x7fffffff || width > 0x3fffffff)
+        return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, heads and tokens exceed one launch");
+    const hipError_t e = launch_kv_read(lane, layout, first, tokens, k, v);
+    if (e != hipSuccess) return hip_fail(e, op, lane->device, "cache read launch");
+    lane->counters.kernel_launches += 1;
+    return NNHIP_OK;
+}
+
+int nnhip_cached_attention(void* handle, const nnhip_kv_cache* cache, const nnhip_attention_desc* d)
+{
+    const uint32_t op = NNHIP_OP_ATTENTION;
+    NNHIP_LANE(handle, op)
+    KvLayout layout;
+    int rc = kv_cache_of(op, lane, cache, &layout);
+    if (rc != NNHIP_OK) return rc;
+    if (!d || d->struct_size != sizeof(nnhip_attention_desc))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "descriptor is null or has the wrong struct_size");
+    if (d->tokens < 1 || d->heads < 1 || d->heads % layout.kv_heads != 0)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive and heads a positive multiple of kv_heads");
+    if (d->window < 0 || d->sinks < 0)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "window and sinks must not be negative");
+    if (!(d->scale >= 0.0f) || !std::isfinite(d->scale))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "scale must be finite and not negative");
+    const int64_t width = static_cast<int64_t>(d->heads) * layout.head_width;
+    rc = check_rows(op, lane, d->q, layout.sequences, d->tokens, width, false, "q");
+    if (rc == NNHIP_OK) rc = check_rows(op, lane, d->out, layout.sequences, d->tokens, width, true, "out");
+    if (rc != NNHIP_OK) return rc;
+    if (d->q.data == d->out.data) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "out must not overlap q");
+    if (static_cast<__int128>(layout.sequences) * d->tokens * d->heads > 0x7fffffff || width > 0x7fffffff)
+        return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, tokens and heads exceed one launch");
+    const hipError_t e = launch_cached_attention(lane, layout, *d);
+    if (e != hipSuccess) return hip_fail(e, op, lane->device, "attention launch");
+    lane->counters.kernel_launches += 1;
+    return NNHIP_OK;
+}
+
+int nnhip_token_log_probs(void* handle, const nnhip_log_probs_desc* d)
+{
+    const uint32_t op = NNHIP_OP_LOG_PROBS;
+    NNHIP_LANE(handle, op)
+    if (!d || d->struct_size != sizeof(nnhip_log_probs_desc))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "descriptor is null or has the wrong struct_size");
+    if (!d->logits || d->rows < 1 || d->vocabulary < 1)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "logits must be non-null, rows and vocabulary positive");
+    if (d->row_stride < d->vocabulary && !(d->rows == 1 && d->row_stride >= 0))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "row_stride must be at least vocabulary");
+    if (d->top < 0 || d->top > NNHIP_LOG_PROBS_MAX_TOP || d->top > d->vocabulary)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "top must be 0 .. %d and at most vocabulary", NNHIP_LOG_PROBS_MAX_TOP);
+    if ((d->top > 0) != (d->top_ids != nullptr) || (d->top == 0 && d->top_log_probs))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "top_ids and top_log_probs go with a positive top, and top_ids with every one");
+    if ((d->targets != nullptr) != (d->log_probs != nullptr))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "targets and log_probs go together");
+    if (!d->log_probs && !d->entropy && !d->top_ids)
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "nothing to compute");
+    if (d->rows > 65535) return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "rows %d exceeds 65535", d->rows);
+    const hipError_t e = launch_token_log_probs(lane, *d);
+    if (e != hipSuccess) return hip_fail(e, op, lane->device, "log probability launch");
     lane->counters.kernel_launches += 1;
     return NNHIP_OK;
 }

@@ -159,6 +159,14 @@ hipError_t launch_add_in_place(Lane* lane, float* destination, const float* sour
 hipError_t launch_first_token_attention(Lane* lane, const float* v, float* out, int heads, int kv_heads, int head_width);
 hipError_t launch_lora_a(Lane* lane, const float* x, const float* a, float* z, int rows, int width, int rank);
 hipError_t launch_lora_b(Lane* lane, const float* z, const float* b, float* y, int rows, int output, int rank, float scale);
+// 8-bit key/value cache, attention over it, token log probabilities (kv_cache_kernels.hip, attention_kernels.hip,
+// log_prob_kernels.hip).
+struct KvLayout;
+hipError_t launch_kv_store(Lane* lane, const KvLayout& cache, const nnhip_kv_store_desc& d);
+hipError_t launch_kv_advance(Lane* lane, const KvLayout& cache, int tokens, const int32_t* counts);
+hipError_t launch_kv_read(Lane* lane, const KvLayout& cache, const int32_t* first, int tokens, const nnhip_rows& k, const nnhip_rows& v);
+hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d);
+hipError_t launch_token_log_probs(Lane* lane, const nnhip_log_probs_desc& d);
 // Storage types and widths the bf16 prefill mat-mul covers.
 bool matmul_bf16_supported(uint32_t type, int in_w);
 hipError_t launch_fill_u32(Lane* lane, uint32_t* p, uint32_t value, size_t count);

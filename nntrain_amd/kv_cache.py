@@ -1,0 +1,214 @@
+"""QuantizedKvCache: keys and values of a model's attention layers in 8 bits, and attention over them.
+
+One object holds every layer's cache of a batch of sequences and the device array of their lengths.  A step stores its
+tokens layer by layer, attends, and advances the lengths once at the end:
+
+    cache = QuantizedKvCache(lane, layers, sequences, kv_heads, head_width, capacity)
+    for layer in range(layers):
+        cache.store(layer, k, v, tokens, q=q, q_out=q, heads=heads, rotary=rotary)
+        cache.attention(layer, q, heads, tokens, out=context)
+    cache.advance(tokens)
+
+Lengths live on the device, so a captured graph of such a step serves every position.  It stands where the reference's
+attention step keeps its key/value buffers (Qwen35Gpu.AttentionStep, NNtrain.Core/Modules/Qwen35Gpu.Attention.cs:60-120).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from ctypes import byref, c_uint64, c_void_p
+
+import numpy as np
+
+from .lane import HipBuffer, HipExecutionLane
+from .native import (KV_BLOCK_TOKENS, ROTARY_HALVES, ROTARY_PAIRS, AttentionDesc, KvCacheDesc, KvStoreDesc, RowsDesc, check)
+
+
+class Rows:
+    """FP32 rows [sequence, token, width] inside a buffer: element (b, i, c) lies at offset + b * sequence_stride +
+    i * token_stride + c, all in floats.  A plain HipBuffer stands for dense rows."""
+    __slots__ = ("buffer", "token_stride", "sequence_stride", "offset")
+
+    def __init__(self, buffer: HipBuffer, token_stride: int, sequence_stride: int = 0, offset: int = 0):
+        if token_stride < 0 or sequence_stride < 0 or offset < 0:
+            raise ValueError("strides and offset must not be negative.")
+        self.buffer, self.token_stride, self.sequence_stride, self.offset = buffer, token_stride, sequence_stride, offset
+
+
+class Rotary:
+    """Rotary positions: pair j of a head's first `width` components turns by position * inv_freq[j] (inv_freq: FP32 on the
+    device, width / 2 values).  pairs=False: pair j is (j, j + width / 2); pairs=True: (2j, 2j + 1)."""
+    __slots__ = ("inv_freq", "width", "style")
+
+    def __init__(self, inv_freq: HipBuffer, width: int, pairs: bool = False):
+        if width < 2 or width % 2 != 0:
+            raise ValueError("the rotary width must be even and positive.")
+        if inv_freq.nbytes < 2 * width:
+            raise ValueError("inv_freq holds fewer than width / 2 values.")
+        self.inv_freq, self.width, self.style = inv_freq, width, ROTARY_PAIRS if pairs else ROTARY_HALVES
+
+    @staticmethod
+    def frequencies(width: int, base: float = 10000.0) -> np.ndarray:
+        """base^(-2j / width), the usual choice."""
+        return (base ** (-np.arange(0, width, 2, dtype=np.float64) / width)).astype(np.float32)
+
+
+class QuantizedKvCache:
+    BLOCK_TOKENS = KV_BLOCK_TOKENS
+
+    def __init__(self, lane: HipExecutionLane, layers: int, sequences: int, kv_heads: int, head_width: int, capacity: int):
+        if min(layers, sequences, kv_heads, head_width, capacity) <= 0:
+            raise ValueError("layers, sequences, kv_heads, head_width and capacity must be positive.")
+        size = c_uint64()
+        check(lane._lib.nnhip_kv_cache_bytes(sequences, kv_heads, head_width, capacity, byref(size)), "kv_cache_bytes")
+        self.lane, self.layers, self.sequences = lane, layers, sequences
+        self.kv_heads, self.head_width, self.capacity = kv_heads, head_width, capacity
+        self.layer_bytes = size.value
+        self._owned: list[HipBuffer] = []
+        try:
+            self.lengths = lane.allocate_bytes(4 * sequences)
+            self._owned.append(self.lengths)
+            for _ in range(layers):
+                self._owned.append(lane.allocate_bytes(self.layer_bytes))
+        except BaseException:
+            self.dispose()
+            raise
+        self._caches = [KvCacheDesc(ctypes.sizeof(KvCacheDesc), sequences, kv_heads, head_width, capacity, 0, b.ptr, self.lengths.ptr)
+                        for b in self._owned[1:]]
+        self.reset()
+
+    # ---- lengths ----
+    def reset(self) -> None:
+        """Every sequence empty."""
+        self._cache(0)
+        self.lane.fill_u32(self.lengths, 0, self.sequences)
+
+    def set_lengths(self, lengths) -> None:
+        """The tokens each sequence holds; smaller than before drops the last ones."""
+        self._cache(0)
+        values = np.ascontiguousarray(lengths, dtype=np.int32)
+        if values.shape != (self.sequences,) or values.min() < 0 or values.max() > self.capacity:
+            raise ValueError("lengths must be one value of 0 .. capacity for each sequence.")
+        self.lane.write(self.lengths, values)
+
+    def read_lengths(self) -> np.ndarray:
+        self._cache(0)
+        return self.lane.read(self.lengths, np.int32, self.sequences)
+
+    def advance(self, tokens: int = 1, counts: HipBuffer | None = None) -> None:
+        """Adds a step's tokens to the lengths, after its last layer."""
+        cache = self._cache(0)
+        with self.lane.kernel("kv_cache_advance"):
+            check(self.lane._lib.nnhip_kv_cache_advance(self.lane._handle, byref(cache), tokens, self._int32(counts, "counts")),
+                  "kv_cache_advance")
+
+    # ---- tokens ----
+    def store(self, layer: int, k: "HipBuffer | Rows", v: "HipBuffer | Rows", tokens: int = 1, *, counts: HipBuffer | None = None,
+              rotary: Rotary | None = None, q: "HipBuffer | Rows | None" = None, q_out: "HipBuffer | Rows | None" = None,
+              heads: int = 0) -> None:
+        """Stores `tokens` new tokens of every sequence behind its length (the first counts[b] of them with counts, int32 on
+        the device), keys turned by their positions with `rotary`.  q (heads query heads of the same tokens) is turned into
+        q_out, q itself by default.  A sequence whose tokens would pass the capacity is left out."""
+        cache = self._cache(layer)
+        if tokens < 1:
+            raise ValueError("tokens must be positive.")
+        kv_width = self.kv_heads * self.head_width
+        desc = KvStoreDesc(struct_size=ctypes.sizeof(KvStoreDesc), tokens=tokens, counts=self._int32(counts, "counts"),
+                           k=self._rows(k, tokens, kv_width, "k"), v=self._rows(v, tokens, kv_width, "v"))
+        if rotary is not None:
+            if rotary.width > self.head_width:
+                raise ValueError("the rotary width exceeds head_width.")
+            desc.inv_freq, desc.rotary_width, desc.rotary_style = rotary.inv_freq._require(), rotary.width, rotary.style
+        if q is not None:
+            if rotary is None or heads < 1:
+                raise ValueError("q needs rotary and a positive number of heads.")
+            desc.heads = heads
+            desc.q = self._rows(q, tokens, heads * self.head_width, "q")
+            desc.q_out = desc.q if q_out is None else self._rows(q_out, tokens, heads * self.head_width, "q_out")
+        elif q_out is not None or heads:
+            raise ValueError("q_out and heads need q.")
+        with self.lane.kernel("kv_cache_store"):
+            check(self.lane._lib.nnhip_kv_cache_store(self.lane._handle, byref(cache), byref(desc)), "kv_cache_store")
+
+    def attention(self, layer: int, q: "HipBuffer | Rows", heads: int, tokens: int = 1, *, scale: float | None = None,
+                  window: int = 0, sinks: int = 0, counts: HipBuffer | None = None,
+                  out: "HipBuffer | Rows | None" = None) -> "HipBuffer | Rows":
+        """Causal attention of the tokens just stored over the cache: token i of sequence b stands at position lengths[b] + i
+        and sees the keys up to it, with window > 0 the last `window` of them and the first `sinks` tokens.  scale: 1 /
+        sqrt(head_width) by default.  FP32 in and out; rows behind counts[b] are left as they are."""
+        cache = self._cache(layer)
+        if tokens < 1 or heads < 1 or heads % self.kv_heads != 0:
+            raise ValueError("tokens must be positive and heads a positive multiple of kv_heads.")
+        if window < 0 or sinks < 0:
+            raise ValueError("window and sinks must not be negative.")
+        factor = 1.0 / math.sqrt(self.head_width) if scale is None else scale
+        if not math.isfinite(factor) or factor < 0.0:
+            raise ValueError("scale must be finite and not negative.")
+        width = heads * self.head_width
+        rows_in = self._rows(q, tokens, width, "q")
+        target = out if out is not None else self.lane.allocate(self.sequences * tokens * width)
+        try:
+            desc = AttentionDesc(ctypes.sizeof(AttentionDesc), tokens, self._int32(counts, "counts"), rows_in,
+                                 self._rows(target, tokens, width, "out"), heads, min(window, 2**31 - 1), min(sinks, 2**31 - 1), factor)
+            with self.lane.kernel("cached_attention"):
+                check(self.lane._lib.nnhip_cached_attention(self.lane._handle, byref(cache), byref(desc)), "cached_attention")
+        except BaseException:
+            if out is None:
+                target.dispose()
+            raise
+        return target
+
+    def read(self, layer: int, tokens: int, *, first: HipBuffer | None = None, k_out: "HipBuffer | Rows | None" = None,
+             v_out: "HipBuffer | Rows | None" = None) -> None:
+        """FP32 values of tokens first[b] .. first[b] + tokens - 1 of every sequence (first: int32 on the device, 0 without)."""
+        cache = self._cache(layer)
+        if tokens < 1:
+            raise ValueError("tokens must be positive.")
+        if k_out is None and v_out is None:
+            raise ValueError("read needs k_out or v_out.")
+        width = self.kv_heads * self.head_width
+        k = self._rows(k_out, tokens, width, "k_out") if k_out is not None else RowsDesc()
+        v = self._rows(v_out, tokens, width, "v_out") if v_out is not None else RowsDesc()
+        with self.lane.kernel("kv_cache_read"):
+            check(self.lane._lib.nnhip_kv_cache_read(self.lane._handle, byref(cache), self._int32(first, "first"), tokens, byref(k),
+                                                     byref(v)), "kv_cache_read")
+
+    # ---- checks ----
+    def _cache(self, layer: int) -> KvCacheDesc:
+        if not self._owned:
+            raise ValueError("the cache has been disposed")
+        if not 0 <= layer < self.layers:
+            raise IndexError(f"layer {layer} is outside 0 .. {self.layers - 1}.")
+        return self._caches[layer]
+
+    def _int32(self, buffer: HipBuffer | None, name: str) -> c_void_p | None:
+        if buffer is None:
+            return None
+        if buffer.nbytes < 4 * self.sequences:
+            raise ValueError(f"The buffer '{name}' holds fewer values than there are sequences.")
+        return c_void_p(buffer._require())
+
+    def _rows(self, rows: "HipBuffer | Rows", tokens: int, width: int, name: str) -> RowsDesc:
+        if rows is None:
+            raise TypeError(f"{name} is null.")
+        if isinstance(rows, Rows):
+            buffer, token, sequence, offset = rows.buffer, rows.token_stride, rows.sequence_stride, rows.offset
+        else:
+            buffer, token, sequence, offset = rows, width, tokens * width, 0
+        if buffer.nbytes < 4 * (offset + (self.sequences - 1) * sequence + (tokens - 1) * token + width):
+            raise ValueError(f"The buffer '{name}' is too small for its rows.")
+        return RowsDesc(buffer._require() + 4 * offset, token, sequence)
+
+    def dispose(self) -> None:
+        for b in reversed(self._owned):
+            b.dispose()
+        self._owned = []
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.dispose()
+
+
+__all__ = ["QuantizedKvCache", "Rotary", "Rows"]

@@ -134,6 +134,13 @@ class HipExecutionLane:
         check(self._lib.nnhip_alloc(self._handle, nbytes, byref(p)), "alloc")
         return HipBuffer(self, p.value, nbytes)
 
+    def wrap(self, ptr: int, nbytes: int) -> HipBuffer:
+        """A window of device memory that somebody else owns (a torch tensor's data_ptr(), say), for use as an operand of
+        this lane's operations.  The caller keeps it alive and orders its own accesses against the lane's stream."""
+        if ptr <= 0 or nbytes <= 0:
+            raise ValueError("wrap needs a device pointer and a positive size")
+        return _HipBufferView(self, ptr, nbytes)
+
     def trim(self) -> None:
         """Drain the stream and return the blocks kept for reuse to the driver."""
         check(self._lib.nnhip_lane_trim(self._handle), "lane_trim")

@@ -66,6 +66,35 @@ class BatchLaunchInfo(Structure):
                 ("activations_in_lds", c_int32), ("dynamic_lds_bytes", c_int32)]
 
 
+class RowsDesc(Structure):
+    _fields_ = [("data", c_void_p), ("token_stride", c_int64), ("sequence_stride", c_int64)]
+
+
+class KvCacheDesc(Structure):
+    _fields_ = [("struct_size", c_uint32), ("sequences", c_int32), ("kv_heads", c_int32), ("head_width", c_int32),
+                ("capacity", c_int32), ("reserved", c_uint32), ("data", c_void_p), ("lengths", c_void_p)]
+
+
+class KvStoreDesc(Structure):
+    _fields_ = [("struct_size", c_uint32), ("tokens", c_int32), ("counts", c_void_p), ("k", RowsDesc), ("v", RowsDesc),
+                ("q", RowsDesc), ("q_out", RowsDesc), ("inv_freq", c_void_p), ("rotary_width", c_int32),
+                ("rotary_style", c_uint32), ("heads", c_int32), ("reserved", c_uint32)]
+
+
+class AttentionDesc(Structure):
+    _fields_ = [("struct_size", c_uint32), ("tokens", c_int32), ("counts", c_void_p), ("q", RowsDesc), ("out", RowsDesc),
+                ("heads", c_int32), ("window", c_int32), ("sinks", c_int32), ("scale", c_float)]
+
+
+class LogProbsDesc(Structure):
+    _fields_ = [("struct_size", c_uint32), ("rows", c_int32), ("vocabulary", c_int32), ("top", c_int32),
+                ("row_stride", c_int64), ("logits", c_void_p), ("targets", c_void_p), ("log_probs", c_void_p),
+                ("entropy", c_void_p), ("top_ids", c_void_p), ("top_log_probs", c_void_p)]
+
+
+KV_BLOCK_TOKENS = 64
+LOG_PROBS_MAX_TOP = 64
+ROTARY_HALVES, ROTARY_PAIRS = 0, 1
 PRE_NONE, PRE_RMS_NORM, PRE_SILU_MULTIPLY = 0, 1, 2
 POST_NONE, POST_SILU_PAIR = 0, 1
 
@@ -111,6 +140,12 @@ PROTOTYPES = {
     "nnhip_first_token_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int]),
     "nnhip_lora_a": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int]),
     "nnhip_lora_b": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float]),
+    "nnhip_kv_cache_bytes": (c_int, [c_int, c_int, c_int, c_int, POINTER(c_uint64)]),
+    "nnhip_kv_cache_store": (c_int, [c_void_p, POINTER(KvCacheDesc), POINTER(KvStoreDesc)]),
+    "nnhip_kv_cache_advance": (c_int, [c_void_p, POINTER(KvCacheDesc), c_int, c_void_p]),
+    "nnhip_kv_cache_read": (c_int, [c_void_p, POINTER(KvCacheDesc), c_void_p, c_int, POINTER(RowsDesc), POINTER(RowsDesc)]),
+    "nnhip_cached_attention": (c_int, [c_void_p, POINTER(KvCacheDesc), POINTER(AttentionDesc)]),
+    "nnhip_token_log_probs": (c_int, [c_void_p, POINTER(LogProbsDesc)]),
     "nnhip_event_create": (c_int, [c_void_p, POINTER(c_void_p)]),
     "nnhip_event_destroy": (c_int, [c_void_p, c_void_p]),
     "nnhip_event_record": (c_int, [c_void_p, c_void_p]),

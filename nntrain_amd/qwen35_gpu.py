@@ -4,11 +4,13 @@
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from ctypes import c_void_p
+from typing import NamedTuple
 
 from .lane import HipBuffer, HipExecutionLane
-from .native import check
+from .native import LOG_PROBS_MAX_TOP, LogProbsDesc, check
 
 
 def _positive(value: int, name: str) -> None:
@@ -142,8 +144,7 @@ def lora_apply_b(lane: HipExecutionLane, z: HipBuffer, b: HipBuffer, y: HipBuffe
 def first_token_attention(lane: HipExecutionLane, value: HipBuffer, heads: int, kv_heads: int, head_width: int,
                           out: HipBuffer | None = None) -> HipBuffer:
     """Causal grouped-query attention for the first token of a sequence: every query head receives its group's value
-    head (the single key has softmax weight 1).  The general attention step (Qwen35Gpu.AttentionStep) is not part of
-    this library."""
+    head (the single key has softmax weight 1).  Attention over the tokens before it is QuantizedKvCache.attention."""
     _positive(heads, "heads")
     _positive(kv_heads, "kv_heads")
     _positive(head_width, "head_width")
@@ -160,3 +161,56 @@ def first_token_attention(lane: HipExecutionLane, value: HipBuffer, heads: int, 
         if out is None:
             output.dispose()
         raise
+
+
+class TokenLogProbs(NamedTuple):
+    """What token_log_probs leaves on the device; None where it was not asked for."""
+    log_probs: HipBuffer | None       # [rows] FP32
+    entropy: HipBuffer | None         # [rows] FP32
+    top_ids: HipBuffer | None         # [rows, top] int32
+    top_log_probs: HipBuffer | None   # [rows, top] FP32
+
+
+def token_log_probs(lane: HipExecutionLane, logits: HipBuffer, rows: int, vocabulary: int, targets: HipBuffer | None = None,
+                    top: int = 0, row_stride: int | None = None, out: HipBuffer | None = None, entropy: HipBuffer | None = None,
+                    top_ids: HipBuffer | None = None, top_log_probs: HipBuffer | None = None) -> TokenLogProbs:
+    """For every row of logits: the natural log probability of targets[row] (int32), the entropy of the distribution in nats,
+    and the `top` (up to 64) most probable tokens with their log probabilities, the largest first, equal logits by index.
+    Without targets, log_probs is None.  Rows are row_stride floats apart (vocabulary by default)."""
+    _positive(rows, "rows")
+    _positive(vocabulary, "vocabulary")
+    stride = vocabulary if row_stride is None else row_stride
+    if stride < vocabulary:
+        raise ValueError("row_stride must be at least vocabulary.")
+    if not 0 <= top <= min(LOG_PROBS_MAX_TOP, vocabulary):
+        raise ValueError(f"top must be 0 .. {LOG_PROBS_MAX_TOP} and at most vocabulary.")
+    if targets is None and out is not None:
+        raise ValueError("out needs targets.")
+    if not top and (top_ids is not None or top_log_probs is not None):
+        raise ValueError("top_ids and top_log_probs need a positive top.")
+    _validate_buffer(logits, (rows - 1) * stride + vocabulary, "logits")
+    if targets is not None:
+        _validate_buffer(targets, rows, "targets")
+    made: list[HipBuffer] = []
+
+    def output(given: HipBuffer | None, elements: int) -> HipBuffer:
+        buffer = _output(lane, given, elements)
+        if given is None:
+            made.append(buffer)
+        return buffer
+
+    try:
+        out = output(out, rows) if targets is not None else None
+        entropy = output(entropy, rows)
+        if top:
+            top_ids, top_log_probs = output(top_ids, rows * top), output(top_log_probs, rows * top)
+        desc = LogProbsDesc(ctypes.sizeof(LogProbsDesc), rows, vocabulary, top, stride, logits._require(),
+                            targets._require() if targets is not None else None, out._require() if out is not None else None,
+                            entropy._require(), top_ids._require() if top else None, top_log_probs._require() if top else None)
+        with lane.kernel("token_log_probs"):
+            check(lane._lib.nnhip_token_log_probs(lane._handle, ctypes.byref(desc)), "token_log_probs")
+    except BaseException:
+        for buffer in made:
+            buffer.dispose()
+        raise
+    return TokenLogProbs(out, entropy, top_ids, top_log_probs)
