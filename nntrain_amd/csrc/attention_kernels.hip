@@ -1,9 +1,25 @@
 // Attention over the 8-bit key/value cache (nnhip_cached_attention): causal, grouped query heads, optional sliding window
 // with the first tokens kept visible.
 //
-// One wave takes one query row and walks over the blocks of 64 keys with the running maximum m and sum l of the softmax:
+// One pass over the keys with the running maximum m and sum l of the softmax, a block of 64 keys at a time:
 //     s_t = scale q . K_t,   m' = max(m, max_t s_t),   l' = l e^(m - m') + sum_t e^(s_t - m'),   o' = o e^(m - m') + sum_t e^(s_t - m') V_t
-// and writes o / l.  A lane holds the score of one token, then the components d, d + 64, ... of o.
+// and o / l at the end.  All in powers of two: the factor log2(e) goes into the scale.
+//
+// The query rows that share a key/value head (tokens x heads of the group) are the columns of the matrix products, so a block
+// of keys is read once for all of them: S^T = K Q^T, O^T = V^T P^T, on v_mfma_f32_16x16x32_f16 with 16 rows a column tile.
+// Transposed this way a lane's accumulators hold 16 probabilities of one row, in the order in which the cache keeps the
+// values' tokens (kv_cache_layout.h): they are the operand of the second product as they stand, and a row's maximum needs two
+// exchanges between lanes.
+//
+// Precision: the codes are integers up to 127, exact in half precision.  Queries are scaled by a power of two to at most
+// 2^14 and taken as hi + lo half-precision parts, so are the probabilities times (value scale / a running power of two above
+// the value scales) times 2^14: 22 bits below the largest, nothing lost before 2^-38 of it.  Two products for each operand pair
+// instead of one is what FP32 results cost; one rounding to half precision would leave 2^-12.
+//
+// Two kernels.  attend_few_kernel, up to 32 rows a key/value head (decode): bound by reading the cache, so every wave walks over
+// blocks of its own, codes go from memory to registers to half precision without LDS, and the keys are split over many
+// workgroups whose partial results attend_join_kernel adds up.  attend_many_kernel (prompts): bound by the matrix cores, so
+// four waves of 32 rows share each block, converted once into LDS.
 #include "kv_cache_layout.h"
 #include "nnhip_internal.h"
 
@@ -11,82 +27,699 @@ namespace nnhip {
 
 namespace {
 
+constexpr int kThreads = 256, kWaves = 4;
+constexpr float kPartScale = 16384.0f;          // 2^14: probabilities enter the product as p * 2^14
+constexpr float kLeastValueScale = 0x1p-100f;   // keeps kPartScale / (running value scale) finite
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
 struct AttendArgs {
     KvLayout cache;
     int tokens;
     const int32_t* counts;
     nnhip_rows q, out;
-    int heads, window, sinks;
-    float scale;
+    int heads, group;       // group: query heads of a key/value head
+    int window, sinks;
+    float scale;            // times log2(e)
+    bool wide;              // rows of q and out lie on 16-byte boundaries and head_width is a multiple of 4
+    int row_tiles;          // workgroups over the rows of a pair
+    int splits;             // workgroups over the keys
+    int least;              // fewest blocks a split takes
+    float* partial;         // [pair][row][split][padded] sums, then [pair][row][split][2] m, l
+    float* stats;
 };
 
-__global__ __launch_bounds__(64) void attend_row_kernel(const AttendArgs a)
-{
-    __shared__ float query[kKvMaxWidth];
-    __shared__ float prob[kKvBlock];
-    const KvLayout& kv = a.cache;
-    const int lane = threadIdx.x, width = kv.head_width;
-    const unsigned row = blockIdx.x;
-    const int h = static_cast<int>(row % static_cast<unsigned>(a.heads));
-    const int i = static_cast<int>(row / static_cast<unsigned>(a.heads) % static_cast<unsigned>(a.tokens));
-    const int b = static_cast<int>(row / static_cast<unsigned>(a.heads) / static_cast<unsigned>(a.tokens));
-    const int start = kv.lengths[b];
+// The blocks that the rows of one workgroup see: the first `sink_blocks`, then those from `window_block` on.
+struct Span {
+    int start, n;           // tokens before the call, tokens of the call
+    int rows;               // n * group
+    int first, last;        // positions of the first and the last row of the tile
+    int sink_blocks, window_block, blocks;
+    int begin, end;         // of this split
     bool left_out;
-    const int n = kv_tokens_of(start, kv.capacity, a.tokens, a.counts, b, &left_out);
-    if (i >= n) return;
-    const float* q = a.q.data + b * a.q.sequence_stride + i * a.q.token_stride + h * width;
-    float* out = a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * width;
-    if (left_out) {
-        for (int d = lane; d < width; d += 64) out[d] = __uint_as_float(0x7fc00000u);
+    __device__ int block(int index) const { return index < sink_blocks ? index : index - sink_blocks + window_block; }
+};
+
+// Rows [row0, row0 + rows_of_tile) of a pair, split `split`.  The number of splits in use follows from the blocks there are.
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int row0, int rows_of_tile, int split)
+{
+    Span s;
+    s.start = a.cache.lengths[b];
+    s.n = kv_tokens_of(s.start, a.cache.capacity, a.tokens, a.counts, b, &s.left_out);
+    s.rows = s.n * a.group;
+    const int last_row = min(row0 + rows_of_tile, s.rows) - 1;
+    s.first = s.start + row0 / a.group;
+    s.last = s.start + max(last_row, 0) / a.group;
+    const int low = a.window > 0 && s.first >= a.window ? s.first - a.window + 1 : 0;
+    s.window_block = low / kKvBlock;
+    s.sink_blocks = min((min(a.sinks, kKvBlock * s.window_block) + kKvBlock - 1) / kKvBlock, s.window_block);
+    s.blocks = s.sink_blocks + s.last / kKvBlock + 1 - s.window_block;
+    const int each = max(a.least, (s.blocks + a.splits - 1) / a.splits);
+    s.begin = static_cast<int>(min(static_cast<int64_t>(split) * each, static_cast<int64_t>(s.blocks)));
+    s.end = min(s.begin + each, s.blocks);
+    return s;
+}
+
+__device__ __forceinline__ int splits_used(const AttendArgs& a, const Span& s)
+{
+    const int each = max(a.least, (s.blocks + a.splits - 1) / a.splits);
+    return (s.blocks + each - 1) / each;
+}
+
+// Maximum / sum over the four lanes that share a column (lane % 16).
+__device__ __forceinline__ float column_max(float x)
+{
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float column_sum(float x)
+{
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Eight biased codes to half precision: 0x6400 | byte is 1024 + byte, minus 1152 is the code.
+__device__ __forceinline__ half8 halves(uint32_t a, uint32_t b)
+{
+    const half2v bias = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    half2v r[4];
+    r[0] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, a, 0x04010400u)) + bias;
+    r[1] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, a, 0x04030402u)) + bias;
+    r[2] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, b, 0x04010400u)) + bias;
+    r[3] = __builtin_bit_cast(half2v, __builtin_amdgcn_perm(0x64646464u, b, 0x04030402u)) + bias;
+    return __builtin_shufflevector(__builtin_shufflevector(r[0], r[1], 0, 1, 2, 3), __builtin_shufflevector(r[2], r[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// x[0..7] as hi + lo: the nearest half-precision numbers, then those nearest to what is left.
+__device__ __forceinline__ void split_parts(const float* x, half8* hi, half8* lo)
+{
+    half2v h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const floatx2 v = {x[2 * i], x[2 * i + 1]};
+        h[i] = __builtin_convertvector(v, half2v);
+        const floatx2 r = {fmaf(static_cast<float>(h[i].x), -1.0f, v.x), fmaf(static_cast<float>(h[i].y), -1.0f, v.y)};
+        l[i] = __builtin_convertvector(r, half2v);
+    }
+    *hi = __builtin_shufflevector(__builtin_shufflevector(h[0], h[1], 0, 1, 2, 3), __builtin_shufflevector(h[2], h[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+    *lo = __builtin_shufflevector(__builtin_shufflevector(l[0], l[1], 0, 1, 2, 3), __builtin_shufflevector(l[2], l[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ __forceinline__ floatx4 mma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Component at which the eight a lane holds of k-step `step` begin: the order of the key codes.
+template <int DP>
+__device__ __forceinline__ int component_of(int step, int g)
+{
+    return (step / 2 + 1) * 64 <= DP ? step / 2 * 64 + g * 16 + step % 2 * 8 : step / 2 * 64 + g * 8;
+}
+
+// One column tile: 16 query rows and their running softmax.  A lane belongs to row lane % 16.
+template <int DP>
+struct Rows16 {
+    half8 hi[DP / 32], lo[DP / 32];
+    floatx4 o[DP / 16];
+    float c;                // what a product of the scaled query and codes is multiplied by, apart from the key scale
+    float m, l;             // running maximum (in powers of two), this lane's part of the sum
+    int position, low;      // of the row; first key of its window
+
+    __device__ __forceinline__ void load(const AttendArgs& a, const Span& s, int b, int kv_head, int row)
+    {
+        const int lane = threadIdx.x & 63, g = lane >> 4, width = a.cache.head_width;
+        const bool valid = row < s.rows;
+        const int i = valid ? row / a.group : 0, h = valid ? row - i * a.group : 0;
+        const float* q = a.q.data + b * a.q.sequence_stride + i * a.q.token_stride + (kv_head * a.group + h) * width;
+        float x[DP / 32][8];
+        uint32_t most = 0;
+#pragma unroll
+        for (int step = 0; step < DP / 32; ++step) {
+            const int d = component_of<DP>(step, g);
+            if (a.wide) {
+#pragma unroll
+                for (int u = 0; u < 8; u += 4) {
+                    floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if (valid && d + u < width) v = *reinterpret_cast<const floatx4*>(q + d + u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[step][u + e] = v[e];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 8; ++u) x[step][u] = valid && d + u < width ? q[d + u] : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int step = 0; step < DP / 32; ++step)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) most = max(most, __float_as_uint(x[step][u]) & 0x7fffffffu);
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 16)));
+        most = max(most, static_cast<uint32_t>(__shfl_xor(static_cast<int>(most), 32)));
+        // 2^shift brings the largest component into [2^13, 2^14)
+        const int shift = min(13 - (static_cast<int>(most >> 23) - 127), 120);
+        const float up = __uint_as_float(static_cast<uint32_t>(shift + 127) << 23), down = __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+#pragma unroll
+        for (int step = 0; step < DP / 32; ++step) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[step][u] *= up;
+            split_parts(x[step], &hi[step], &lo[step]);
+        }
+        c = most < 0x7f800000u ? a.scale * down : __uint_as_float(0x7fc00000u);
+        m = -INFINITY;
+        l = 0.0f;
+        position = valid ? s.start + i : -1;        // a row that is not there sees nothing
+        low = a.window > 0 && position >= a.window ? position - a.window + 1 : 0;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) o[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // Scores of the block that starts at token t0 -> parts of the probabilities for the second product.
+    //   factor: 2^14 * value scale / running value scale;  keep: running value scale before / after this block
+    template <bool FULL>
+    __device__ __forceinline__ void softmax(floatx4 (&s)[4], int t0, int sinks, float key_scale, float factor, float keep, half8 (&p_hi)[2], half8 (&p_lo)[2])
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+        const float scale = c * key_scale;
+        bool seen[4][4];
+        float top = -INFINITY;
+        if (FULL) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) top = fmaxf(fmaxf(fmaxf(top, s[j][0]), fmaxf(s[j][1], s[j][2])), s[j][3]);
+            top *= scale;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + 16 * j + 4 * g + i;
+                    seen[j][i] = t <= position && (t >= low || t < sinks);
+                    s[j][i] *= scale;
+                    top = seen[j][i] ? fmaxf(top, s[j][i]) : top;
+                }
+        }
+        const float next = fmaxf(m, column_max(top)), base = next == -INFINITY ? 0.0f : next;
+        if (keep != 1.0f || __any(next > m)) {
+            const float shrink = __builtin_amdgcn_exp2f(m - base);
+            l *= shrink;
+            const float all = shrink * keep;
+#pragma unroll
+            for (int t = 0; t < DP / 16; ++t) o[t] *= all;
+        }
+        m = next;
+        float sum = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float w[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int j = 2 * h + u / 4, i = u % 4;
+                float p;
+                if (FULL) {
+                    p = __builtin_amdgcn_exp2f(fmaf(s[j][i], scale, -base));
+                    w[u] = p * factor;
+                } else {
+                    p = seen[j][i] ? __builtin_amdgcn_exp2f(s[j][i] - base) : 0.0f;
+                    w[u] = seen[j][i] ? p * factor : 0.0f;
+                }
+                sum += p;
+            }
+            split_parts(w, &p_hi[h], &p_lo[h]);
+        }
+        l += sum;
+    }
+};
+
+// A block whose every token every row of [first, last] sees.
+__device__ __forceinline__ bool sees_all(const AttendArgs& a, int t0, int first, int last)
+{
+    return t0 + kKvBlock - 1 <= first && (a.window == 0 || t0 > last - a.window || t0 + kKvBlock - 1 < a.sinks);
+}
+
+// The running power of two above the value scales of the blocks so far.
+__device__ __forceinline__ float above(float value_scale, float running)
+{
+    const uint32_t bits = __float_as_uint(value_scale);
+    if ((bits & 0x7f800000u) == 0x7f800000u) return running;        // NaN: the probabilities carry it
+    return fmaxf(running, __uint_as_float((bits & 0x7f800000u) + 0x00800000u));
+}
+
+__device__ __forceinline__ void put(float* to, floatx4 v, int d, int width, bool wide)
+{
+    if (wide) {
+        if (d < width) *reinterpret_cast<floatx4*>(to + d) = v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (d + e < width) to[d + e] = v[e];
+    }
+}
+
+// Rows of sequences that are left out become NaN.
+__device__ void refuse_rows(const AttendArgs& a, const Span& s, int b, int kv_head, int row0, int rows)
+{
+    for (int e = threadIdx.x; e < rows * a.cache.head_width; e += kThreads) {
+        const int row = row0 + e / a.cache.head_width, d = e % a.cache.head_width;
+        if (row >= s.rows) break;
+        const int i = row / a.group, h = kv_head * a.group + row % a.group;
+        a.out.data[b * a.out.sequence_stride + i * a.out.token_stride + h * a.cache.head_width + d] = __uint_as_float(0x7fc00000u);
+    }
+}
+
+template <int DP>
+struct Codes {
+    static constexpr int kWhole = DP / 64, kRest = DP % 64 ? 1 : 0;
+    uint4 k[kWhole ? kWhole * 4 : 1], v[DP / 16];
+    uint2 rest[4];
+    float2 scales;
+
+    __device__ __forceinline__ void load_keys(const KvLayout& kv, int pair, int block, int lane)
+    {
+        const uint8_t* at = kv.codes(0, pair, block);
+#pragma unroll
+        for (int u = 0; u < kWhole * 4; ++u) k[u] = *reinterpret_cast<const uint4*>(at + u * 1024 + lane * 16);
+        if (kRest) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rest[j] = *reinterpret_cast<const uint2*>(at + kWhole * 4096 + j * 512 + lane * 8);
+        }
+        scales = *reinterpret_cast<const float2*>(kv.scales(pair, block));
+    }
+    __device__ __forceinline__ void load_values(const KvLayout& kv, int pair, int block, int lane)
+    {
+        const uint8_t* at = kv.codes(1, pair, block);
+#pragma unroll
+        for (int u = 0; u < DP / 16; ++u) v[u] = *reinterpret_cast<const uint4*>(at + u * 1024 + lane * 16);
+    }
+    __device__ __forceinline__ half8 key(int step, int j) const
+    {
+        if (step / 2 < kWhole) {
+            const uint4& x = k[step / 2 * 4 + j];
+            return step % 2 ? halves(x.z, x.w) : halves(x.x, x.y);
+        }
+        return halves(rest[j].x, rest[j].y);
+    }
+    __device__ __forceinline__ half8 value(int t, int h) const { return h ? halves(v[t].z, v[t].w) : halves(v[t].x, v[t].y); }
+};
+
+template <int DP, int CT>
+__global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_kernel(const AttendArgs a)
+{
+    constexpr int kRows = CT * 16, kPitch = DP + 4;
+    __shared__ float sums[2][kRows * kPitch];
+    __shared__ float stats[kWaves][kRows][2];
+    const KvLayout& kv = a.cache;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    unsigned at = blockIdx.x;
+    const int split = static_cast<int>(at % static_cast<unsigned>(a.splits));
+    at /= static_cast<unsigned>(a.splits);
+    const int row0 = static_cast<int>(at % static_cast<unsigned>(a.row_tiles)) * kRows, pair = static_cast<int>(at / static_cast<unsigned>(a.row_tiles));
+    const int b = pair / kv.kv_heads, kv_head = pair - b * kv.kv_heads;
+    const Span s = span_of(a, b, row0, kRows, split);
+    if (row0 >= s.rows) return;
+    if (s.left_out) {
+        if (split == 0) refuse_rows(a, s, b, kv_head, row0, kRows);
         return;
     }
-    const int pair = b * kv.kv_heads + h / (a.heads / kv.kv_heads), p = start + i;
-    const int low = a.window > 0 && p >= a.window ? p - a.window + 1 : 0;       // first key of the window
-    for (int d = lane; d < width; d += 64) query[d] = q[d];
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[kKvMaxWidth / 64] = {};
-    for (int block = 0; block * kKvBlock <= p; ++block) {
-        if (block * kKvBlock + kKvBlock <= low && block * kKvBlock >= a.sinks) {
-            block = low / kKvBlock - 1;
-            continue;
+    if (s.begin >= s.end) return;
+
+    Rows16<DP> r[CT];
+    Codes<DP> codes;
+    int index = s.begin + wave;
+    if (index < s.end) {
+        codes.load_keys(kv, pair, s.block(index), lane);
+        codes.load_values(kv, pair, s.block(index), lane);
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) r[t].load(a, s, b, kv_head, row0 + t * 16 + (lane & 15));
+    float running = kLeastValueScale;
+    while (index < s.end) {
+        const int t0 = s.block(index) * kKvBlock;
+        floatx4 scores[CT][4];
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) scores[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int step = 0; step < DP / 32; ++step)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const half8 k = codes.key(step, j);
+#pragma unroll
+                for (int t = 0; t < CT; ++t) {
+                    scores[t][j] = mma(k, r[t].hi[step], scores[t][j]);
+                    scores[t][j] = mma(k, r[t].lo[step], scores[t][j]);
+                }
+            }
+        const float2 scales = codes.scales;
+        index += kWaves;
+        const int next = s.block(min(index, s.end - 1));
+        if (index < s.end) codes.load_keys(kv, pair, next, lane);
+        const float higher = above(scales.y, running), keep = running / higher, factor = scales.y * (kPartScale / higher);
+        running = higher;
+        const bool full = sees_all(a, t0, s.first, s.last);
+        half8 p_hi[CT][2], p_lo[CT][2];
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            if (full)
+                r[t].template softmax<true>(scores[t], t0, a.sinks, scales.x, factor, keep, p_hi[t], p_lo[t]);
+            else
+                r[t].template softmax<false>(scores[t], t0, a.sinks, scales.x, factor, keep, p_hi[t], p_lo[t]);
         }
-        const int t = block * kKvBlock + lane;
-        const bool seen = t <= p && (t >= low || t < a.sinks);
-        const float* scales = kv.scales(pair, block);
-        const uint8_t* k = kv.codes(0, pair, block);
-        float s = 0.0f;
-        for (int d = 0; d < width; ++d) s = fmaf(query[d], static_cast<float>(k[kv_key_offset(kv.padded, lane, d)] - 128), s);
-        s = s * scales[0] * a.scale;
-        float top = seen ? s : -INFINITY;
-        for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-        const float next = fmaxf(m, top), base = next == -INFINITY ? 0.0f : next;
-        const float keep = expf(m - base), e = seen ? expf(s - base) : 0.0f;
-        m = next;
-        prob[lane] = seen ? e * scales[1] : 0.0f;
-        __syncthreads();
-        l = l * keep + e;
-        const uint8_t* v = kv.codes(1, pair, block);
-        for (int c = 0; c * 64 < width; ++c) {
-            o[c] *= keep;
-            const int d = c * 64 + lane;
-            if (d >= width) continue;
-            for (int u = 0; u < kKvBlock; ++u)
-                if (prob[u] != 0.0f) o[c] = fmaf(prob[u], static_cast<float>(v[kv_value_offset(u, d)] - 128), o[c]);
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const half8 v = codes.value(d, h);
+#pragma unroll
+                for (int t = 0; t < CT; ++t) {
+                    r[t].o[d] = mma(v, p_hi[t][h], r[t].o[d]);
+                    r[t].o[d] = mma(v, p_lo[t][h], r[t].o[d]);
+                }
+            }
+        if (index < s.end) codes.load_values(kv, pair, next, lane);
+    }
+    // the four waves' sums, in a fixed order: 0 + 2 and 1 + 3 through LDS, then the two
+    const int column = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        r[t].l = column_sum(r[t].l);
+        if (g == 0) {
+            stats[wave][t * 16 + column][0] = r[t].m;
+            stats[wave][t * 16 + column][1] = r[t].l;
+        }
+    }
+    __syncthreads();
+    for (int round = 0; round < 2; ++round) {
+        if (wave / 2 == round) {
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                const int row = t * 16 + column;
+                float m = stats[0][row][0];
+                for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[w][row][0]);
+                const float factor = __builtin_amdgcn_exp2f(r[t].m - (m == -INFINITY ? 0.0f : m)) * (running * (1.0f / kPartScale));
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) {
+                    floatx4* to = reinterpret_cast<floatx4*>(&sums[wave & 1][row * kPitch + d * 16 + g * 4]);
+                    const floatx4 x = r[t].o[d] * factor;
+                    *to = round ? *to + x : x;
+                }
+            }
         }
         __syncthreads();
     }
+    const int used = splits_used(a, s);
+    for (int e = threadIdx.x; e < kRows * (DP / 4); e += kThreads) {
+        const int row = e / (DP / 4), d = e % (DP / 4) * 4;
+        if (row0 + row >= s.rows) break;
+        float m = stats[0][row][0], l = 0.0f;
+        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[w][row][0]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        for (int w = 0; w < kWaves; ++w) l += stats[w][row][1] * __builtin_amdgcn_exp2f(stats[w][row][0] - base);
+        floatx4 x = *reinterpret_cast<const floatx4*>(&sums[0][row * kPitch + d]) + *reinterpret_cast<const floatx4*>(&sums[1][row * kPitch + d]);
+        if (used == 1) {
+            const int i = (row0 + row) / a.group, h = kv_head * a.group + (row0 + row) % a.group;
+            x /= l;
+            put(a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * kv.head_width, x, d, kv.head_width, a.wide);
+        } else {
+            const size_t to = (static_cast<size_t>(pair) * a.tokens * a.group + row0 + row) * a.splits + split;
+            *reinterpret_cast<floatx4*>(a.partial + to * DP + d) = x;
+            if (d == 0) {
+                a.stats[2 * to] = m;
+                a.stats[2 * to + 1] = l;
+            }
+        }
+    }
+}
+
+// 128 rows, 32 a wave; blocks staged in LDS as half precision in operand order (every fragment 1 KB in lane order: no bank is
+// asked twice), two buffers, one barrier a block; the next block's codes travel during the products.
+template <int DP>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_many_kernel(const AttendArgs a)
+{
+    constexpr int CT = 2, kRows = CT * 16 * kWaves, kUnits = DP * kKvBlock / 16, kPerThread = (kUnits + kThreads - 1) / kThreads;
+    constexpr int kWhole = DP / 64, kFragments = DP * kKvBlock * 2 / 1024;       // KB of keys (or values) in half precision
+    extern __shared__ uint4 staged[];                                            // [2][keys, values][fragment][64]
+    const KvLayout& kv = a.cache;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    // the tiles with the longest spans first, the pairs side by side
+    const int pairs = kv.sequences * kv.kv_heads;
+    unsigned at = blockIdx.x;
+    const int pair = static_cast<int>(at % static_cast<unsigned>(pairs));
+    at /= static_cast<unsigned>(pairs);
+    const int split = static_cast<int>(at % static_cast<unsigned>(a.splits)), row0 = (a.row_tiles - 1 - static_cast<int>(at / static_cast<unsigned>(a.splits))) * kRows;
+    const int b = pair / kv.kv_heads, kv_head = pair - b * kv.kv_heads;
+    const Span s = span_of(a, b, row0, kRows, split);
+    if (row0 >= s.rows) return;
+    if (s.left_out) {
+        if (split == 0) refuse_rows(a, s, b, kv_head, row0, kRows);
+        return;
+    }
+    if (s.begin >= s.end) return;
+
+    uint4 keys[kPerThread], values[kPerThread];
+    float2 scales = {0.0f, 0.0f}, scales_next;
+    auto fetch = [&](int index) {
+        const int block = s.block(index);
+        const uint4* k = reinterpret_cast<const uint4*>(kv.codes(0, pair, block));
+        const uint4* v = reinterpret_cast<const uint4*>(kv.codes(1, pair, block));
+#pragma unroll
+        for (int u = 0; u < kPerThread; ++u)
+            if (kUnits % kThreads == 0 || tid + u * kThreads < kUnits) {
+                keys[u] = k[tid + u * kThreads];
+                values[u] = v[tid + u * kThreads];
+            }
+        scales_next = *reinterpret_cast<const float2*>(kv.scales(pair, block));
+    };
+    // 16 codes of a unit are two lanes' or two steps' fragments
+    auto stage = [&](int buffer) {
+        uint4* k = staged + buffer * 2 * kFragments * 64;
+        uint4* v = k + kFragments * 64;
+#pragma unroll
+        for (int u = 0; u < kPerThread; ++u) {
+            const int unit = tid + u * kThreads;
+            if (kUnits % kThreads != 0 && unit >= kUnits) break;
+            const uint4 x0 = __builtin_bit_cast(uint4, halves(keys[u].x, keys[u].y)), x1 = __builtin_bit_cast(uint4, halves(keys[u].z, keys[u].w));
+            if (unit < kWhole * 256) {                              // [chunk][j][lane]: steps 2 chunk, 2 chunk + 1
+                const int chunk = unit >> 8, j = unit >> 6 & 3, l = unit & 63;
+                k[((2 * chunk) * 4 + j) * 64 + l] = x0;
+                k[((2 * chunk + 1) * 4 + j) * 64 + l] = x1;
+            } else {                                                // [j][lane pair]: the last step
+                const int rest = unit - kWhole * 256;
+                k[(2 * kWhole * 4) * 64 + 2 * rest] = x0;
+                k[(2 * kWhole * 4) * 64 + 2 * rest + 1] = x1;
+            }
+            v[(unit >> 6) * 128 + (unit & 63)] = __builtin_bit_cast(uint4, halves(values[u].x, values[u].y));
+            v[(unit >> 6) * 128 + 64 + (unit & 63)] = __builtin_bit_cast(uint4, halves(values[u].z, values[u].w));
+        }
+        scales = scales_next;
+    };
+
+    fetch(s.begin);
+    Rows16<DP> r[CT];
+    const int row_of_wave = row0 + wave * CT * 16;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) r[t].load(a, s, b, kv_head, row_of_wave + t * 16 + (lane & 15));
+    // positions of this wave's rows, for what it may skip
+    const int first = s.start + min(row_of_wave, s.rows - 1) / a.group, last = s.start + (min(row_of_wave + CT * 16, s.rows) - 1) / a.group;
+    const int low = a.window > 0 && first >= a.window ? first - a.window + 1 : 0;
+    const bool any_row = row_of_wave < s.rows;
+    float running = kLeastValueScale;
+    stage(0);
+    __syncthreads();
+    for (int index = s.begin; index < s.end; ++index) {
+        const int buffer = (index - s.begin) & 1, t0 = s.block(index) * kKvBlock;
+        const float2 now = scales;
+        if (index + 1 < s.end) fetch(index + 1);
+        if (any_row && t0 <= last && (t0 + kKvBlock > low || t0 < a.sinks)) {
+            const uint4* k = staged + buffer * 2 * kFragments * 64 + lane;
+            const uint4* v = k + kFragments * 64;
+            floatx4 scores[CT][4];
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) scores[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int step = 0; step < DP / 32; ++step)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const half8 x = __builtin_bit_cast(half8, k[(step * 4 + j) * 64]);
+#pragma unroll
+                    for (int t = 0; t < CT; ++t) {
+                        scores[t][j] = mma(x, r[t].hi[step], scores[t][j]);
+                        scores[t][j] = mma(x, r[t].lo[step], scores[t][j]);
+                    }
+                }
+            const float higher = above(now.y, running), keep = running / higher, factor = now.y * (kPartScale / higher);
+            running = higher;
+            const bool full = sees_all(a, t0, first, last);
+            half8 p_hi[CT][2], p_lo[CT][2];
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+                if (full)
+                    r[t].template softmax<true>(scores[t], t0, a.sinks, now.x, factor, keep, p_hi[t], p_lo[t]);
+                else
+                    r[t].template softmax<false>(scores[t], t0, a.sinks, now.x, factor, keep, p_hi[t], p_lo[t]);
+            }
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const half8 x = __builtin_bit_cast(half8, v[(d * 2 + h) * 64]);
+#pragma unroll
+                    for (int t = 0; t < CT; ++t) {
+                        r[t].o[d] = mma(x, p_hi[t][h], r[t].o[d]);
+                        r[t].o[d] = mma(x, p_lo[t][h], r[t].o[d]);
+                    }
+                }
+        }
+        if (index + 1 < s.end) stage(buffer ^ 1);
+        __syncthreads();
+    }
+    const int used = splits_used(a, s), g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        const float l = column_sum(r[t].l);
+        const int row = row_of_wave + t * 16 + (lane & 15);
+        if (row >= s.rows) continue;
+        if (used == 1) {
+            const int i = row / a.group, h = kv_head * a.group + row % a.group;
+            float* to = a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * kv.head_width;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) put(to, r[t].o[d] * (running * (1.0f / kPartScale)) / l, d * 16 + g * 4, kv.head_width, a.wide);
+        } else {
+            const size_t to = (static_cast<size_t>(pair) * a.tokens * a.group + row) * a.splits + split;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                *reinterpret_cast<floatx4*>(a.partial + to * DP + d * 16 + g * 4) = r[t].o[d] * (running * (1.0f / kPartScale));
+            if (g == 0) {
+                a.stats[2 * to] = r[t].m;
+                a.stats[2 * to + 1] = l;
+            }
+        }
+    }
+}
+
+// Adds up the splits of one row: sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k, in the order of the splits within each of the
+// eight groups, then of the groups.
+__global__ __launch_bounds__(kThreads) void attend_join_kernel(const AttendArgs a, int rows_of_tile)
+{
+    __shared__ floatx4 sums[kThreads];
+    __shared__ float tops[kWaves], totals[kWaves];
+    const KvLayout& kv = a.cache;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const unsigned rows = static_cast<unsigned>(a.tokens) * static_cast<unsigned>(a.group);
+    const int row = static_cast<int>(blockIdx.x % rows), pair = static_cast<int>(blockIdx.x / rows);
+    const int b = pair / kv.kv_heads, kv_head = pair - b * kv.kv_heads;
+    const Span s = span_of(a, b, row / rows_of_tile * rows_of_tile, rows_of_tile, 0);
+    if (row >= s.rows || s.left_out) return;
+    const int used = splits_used(a, s);
+    if (used == 1) return;
+    const size_t from = static_cast<size_t>(blockIdx.x) * a.splits;
+    float m = -INFINITY;
+    for (int k = tid; k < used; k += kThreads) m = fmaxf(m, a.stats[2 * (from + k)]);
+    for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if (lane == 0) tops[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    for (int k = tid; k < used; k += kThreads) l += a.stats[2 * (from + k) + 1] * __builtin_amdgcn_exp2f(a.stats[2 * (from + k)] - base);
     for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
-    for (int c = 0; c * 64 < width; ++c)
-        if (c * 64 + lane < width) out[c * 64 + lane] = o[c] / l;
+    if (lane == 0) totals[wave] = l;
+    __syncthreads();
+    l = (totals[0] + totals[1]) + (totals[2] + totals[3]);
+    const int i = row / a.group, h = kv_head * a.group + row % a.group;
+    float* out = a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * kv.head_width;
+    for (int d0 = 0; d0 < kv.padded; d0 += 128) {
+        const int d = d0 + (tid & 31) * 4;
+        floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (d < kv.padded)
+            for (int k = tid >> 5; k < used; k += 8)
+                x += *reinterpret_cast<const floatx4*>(a.partial + (from + k) * kv.padded + d) * __builtin_amdgcn_exp2f(a.stats[2 * (from + k)] - base);
+        sums[tid] = x;
+        __syncthreads();
+        if (tid < 32 && d < kv.padded) {
+            for (int k = 1; k < 8; ++k) x += sums[tid + 32 * k];
+            put(out, x / l, d, kv.head_width, a.wide);
+        }
+        __syncthreads();
+    }
+}
+
+template <int DP>
+hipError_t launch(Lane* lane, AttendArgs& a, bool few, int tiles)
+{
+    const unsigned groups = static_cast<unsigned>(a.cache.sequences) * static_cast<unsigned>(a.cache.kv_heads) * static_cast<unsigned>(a.row_tiles) * static_cast<unsigned>(a.splits);
+    if (few) {
+        if (tiles == 1)
+            hipLaunchKernelGGL((attend_few_kernel<DP, 1>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
+        else
+            hipLaunchKernelGGL((attend_few_kernel<DP, 2>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
+        return hipGetLastError();
+    }
+    constexpr int kLds = 2 * 2 * DP * kKvBlock * 2;
+    static LdsLimit limit;
+    const hipError_t e = limit.ensure(lane->device, reinterpret_cast<const void*>(&attend_many_kernel<DP>), kLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(attend_many_kernel<DP>, dim3(groups), dim3(kThreads), kLds, lane->stream, a);
+    return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d)
+// Splits of the keys and scratch floats for a call; the caller provides the scratch memory.
+AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_desc& d, int compute_units)
 {
-    const AttendArgs a{cache, d.tokens, d.counts, d.q, d.out, d.heads, d.window, d.sinks, d.scale};
-    hipLaunchKernelGGL(attend_row_kernel, dim3(static_cast<unsigned>(cache.sequences) * static_cast<unsigned>(d.tokens) * static_cast<unsigned>(d.heads)),
-                       dim3(64), 0, lane->stream, a);
+    AttendPlan p{};
+    const int64_t rows = static_cast<int64_t>(d.tokens) * (d.heads / cache.kv_heads);
+    p.few = rows <= 32;
+    p.rows_of_tile = p.few ? (rows <= 16 ? 16 : 32) : 128;
+    p.row_tiles = static_cast<int>((rows + p.rows_of_tile - 1) / p.rows_of_tile);
+    // blocks a tile of rows can see at most
+    int64_t blocks = cache.blocks;
+    if (d.window > 0) {
+        const int64_t seen = (static_cast<int64_t>(d.window) + p.rows_of_tile / (d.heads / cache.kv_heads) + 1) / kKvBlock + 2 +
+                             (static_cast<int64_t>(d.sinks) + kKvBlock - 1) / kKvBlock;
+        blocks = blocks < seen ? blocks : seen;
+    }
+    p.least = p.few ? kWaves : 8;
+    const int64_t groups = static_cast<int64_t>(cache.sequences) * cache.kv_heads * p.row_tiles;
+    int64_t splits = (2 * 2 * static_cast<int64_t>(compute_units) + groups - 1) / groups;
+    const int64_t most = (blocks + p.least - 1) / p.least;
+    if (splits > most) splits = most;
+    p.splits = static_cast<int>(splits < 1 ? 1 : splits);
+    if (p.splits > 1) {
+        p.stats_at = static_cast<size_t>(cache.sequences) * cache.kv_heads * rows * p.splits * cache.padded;
+        p.scratch_floats = p.stats_at + static_cast<size_t>(cache.sequences) * cache.kv_heads * rows * p.splits * 2;
+    }
+    return p;
+}
+
+hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d, const AttendPlan& p, float* scratch)
+{
+    AttendArgs a{cache, d.tokens, d.counts, d.q, d.out, d.heads, d.heads / cache.kv_heads, d.window, d.sinks, d.scale * 1.44269504088896340736f, false, p.row_tiles,
+                 p.splits, p.least, scratch, scratch ? scratch + p.stats_at : nullptr};
+    auto aligned = [](const nnhip_rows& r) {
+        return (reinterpret_cast<uintptr_t>(r.data) & 15u) == 0 && r.token_stride % 4 == 0 && r.sequence_stride % 4 == 0;
+    };
+    a.wide = cache.head_width % 4 == 0 && aligned(d.q) && aligned(d.out);
+    const int tiles = p.rows_of_tile / 16;
+    hipError_t e;
+    switch (cache.padded) {
+    case 32: e = launch<32>(lane, a, p.few, tiles); break;
+    case 64: e = launch<64>(lane, a, p.few, tiles); break;
+    case 96: e = launch<96>(lane, a, p.few, tiles); break;
+    case 128: e = launch<128>(lane, a, p.few, tiles); break;
+    case 192: e = launch<192>(lane, a, p.few, tiles); break;
+    default: e = launch<256>(lane, a, p.few, tiles); break;
+    }
+    if (e != hipSuccess || p.splits == 1) return e;
+    hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>(cache.sequences) * static_cast<unsigned>(d.tokens) * static_cast<unsigned>(d.heads)),
+                       dim3(kThreads), 0, lane->stream, a, p.rows_of_tile);
     return hipGetLastError();
 }
 

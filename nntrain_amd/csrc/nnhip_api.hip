@@ -884,9 +884,18 @@ int nnhip_cached_attention(void* handle, const nnhip_kv_cache* cache, const nnhi
     if (d->q.data == d->out.data) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "out must not overlap q");
     if (static_cast<__int128>(layout.sequences) * d->tokens * d->heads > 0x7fffffff || width > 0x7fffffff)
         return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, tokens and heads exceed one launch");
-    const hipError_t e = launch_cached_attention(lane, layout, *d);
+    // partial results of the splits live in a lane block for the duration of the two launches
+    const AttendPlan plan = plan_cached_attention(layout, *d, lane->compute_units);
+    void* scratch = nullptr;
+    if (plan.scratch_floats) {
+        rc = nnhip_alloc(handle, plan.scratch_floats * sizeof(float), &scratch);
+        if (rc != NNHIP_OK) return rc;
+    }
+    const hipError_t e = launch_cached_attention(lane, layout, *d, plan, static_cast<float*>(scratch));
+    const int freed = scratch ? nnhip_free(handle, scratch) : NNHIP_OK;
     if (e != hipSuccess) return hip_fail(e, op, lane->device, "attention launch");
-    lane->counters.kernel_launches += 1;
+    if (freed != NNHIP_OK) return freed;
+    lane->counters.kernel_launches += plan.splits > 1 ? 2 : 1;
     return NNHIP_OK;
 }
 

@@ -165,7 +165,14 @@ struct KvLayout;
 hipError_t launch_kv_store(Lane* lane, const KvLayout& cache, const nnhip_kv_store_desc& d);
 hipError_t launch_kv_advance(Lane* lane, const KvLayout& cache, int tokens, const int32_t* counts);
 hipError_t launch_kv_read(Lane* lane, const KvLayout& cache, const int32_t* first, int tokens, const nnhip_rows& k, const nnhip_rows& v);
-hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d);
+// How an attention call is cut up (from its sizes alone, so that a captured graph keeps its form), and its scratch memory.
+struct AttendPlan {
+    bool few;               // up to 32 query rows a key/value head
+    int rows_of_tile, row_tiles, splits, least;
+    size_t scratch_floats, stats_at;
+};
+AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_desc& d, int compute_units);
+hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d, const AttendPlan& plan, float* scratch);
 hipError_t launch_token_log_probs(Lane* lane, const nnhip_log_probs_desc& d);
 // Storage types and widths the bf16 prefill mat-mul covers.
 bool matmul_bf16_supported(uint32_t type, int in_w);
