@@ -117,19 +117,27 @@ __device__ __forceinline__ half8 halves(uint32_t a, uint32_t b)
     return __builtin_shufflevector(__builtin_shufflevector(r[0], r[1], 0, 1, 2, 3), __builtin_shufflevector(r[2], r[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// x[0..7] as hi + lo: the nearest half-precision numbers, then those nearest to what is left.
-__device__ __forceinline__ void split_parts(const float* x, half8* hi, half8* lo)
+// x[0..7] as hi + lo: the nearest half-precision numbers, then those nearest to what is left.  `minus` is -1 in a register: the
+// difference is then one instruction that reads the half-precision number as it stands.
+__device__ __forceinline__ void split_parts(const float* x, float minus, half8* hi, half8* lo)
 {
     half2v h[4], l[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const floatx2 v = {x[2 * i], x[2 * i + 1]};
         h[i] = __builtin_convertvector(v, half2v);
-        const floatx2 r = {fmaf(static_cast<float>(h[i].x), -1.0f, v.x), fmaf(static_cast<float>(h[i].y), -1.0f, v.y)};
+        const floatx2 r = {fmaf(static_cast<float>(h[i].x), minus, v.x), fmaf(static_cast<float>(h[i].y), minus, v.y)};
         l[i] = __builtin_convertvector(r, half2v);
     }
     *hi = __builtin_shufflevector(__builtin_shufflevector(h[0], h[1], 0, 1, 2, 3), __builtin_shufflevector(h[2], h[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
     *lo = __builtin_shufflevector(__builtin_shufflevector(l[0], l[1], 0, 1, 2, 3), __builtin_shufflevector(l[2], l[3], 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+__device__ __forceinline__ float minus_one()
+{
+    float x = -1.0f;
+    asm volatile("" : "+v"(x));
+    return x;
 }
 
 __device__ __forceinline__ floatx4 mma(half8 a, half8 b, floatx4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -187,85 +195,95 @@ struct Rows16 {
         for (int step = 0; step < DP / 32; ++step) {
 #pragma unroll
             for (int u = 0; u < 8; ++u) x[step][u] *= up;
-            split_parts(x[step], &hi[step], &lo[step]);
+            split_parts(x[step], -1.0f, &hi[step], &lo[step]);
         }
-        c = most < 0x7f800000u ? a.scale * down : __uint_as_float(0x7fc00000u);
+        c = most < 0x7f800000u ? a.scale * down : 0.0f;
         m = -INFINITY;
-        l = 0.0f;
+        l = most < 0x7f800000u ? 0.0f : __uint_as_float(0x7fc00000u);           // (a query that is not finite: its row is NaN)
         position = valid ? s.start + i : -1;        // a row that is not there sees nothing
         low = a.window > 0 && position >= a.window ? position - a.window + 1 : 0;
 #pragma unroll
         for (int t = 0; t < DP / 16; ++t) o[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // Scores of the block that starts at token t0 -> parts of the probabilities for the second product.
-    //   factor: 2^14 * value scale / running value scale;  keep: running value scale before / after this block
-    template <bool FULL>
-    __device__ __forceinline__ void softmax(floatx4 (&s)[4], int t0, int sinks, float key_scale, float factor, float keep, half8 (&p_hi)[2], half8 (&p_lo)[2])
-    {
-        const int g = (threadIdx.x & 63) >> 4;
-        const float scale = c * key_scale;
-        bool seen[4][4];
-        float top = -INFINITY;
-        if (FULL) {
+    // Whether the row sees any token of the block that starts at t0, whether it sees token t.
+    __device__ __forceinline__ bool sees_block(int t0, int sinks) const { return t0 <= position && (t0 + kKvBlock > low || t0 < sinks); }
+    __device__ __forceinline__ bool sees(int t, int sinks) const { return t <= position && (t >= low || t < sinks); }
+};
+
+// The softmax step of one block for CT column tiles: scores (products of scaled queries and codes) -> parts of the
+// probabilities for the second product; m, l and o of the rows move on.  `running` is the power of two that the sums o are
+// scaled by, the least one seen so far above the value scales.
+template <int DP, int CT>
+__device__ __forceinline__ void softmax_step(Rows16<DP> (&r)[CT], floatx4 (&s)[CT][4], float2 scales, int t0, bool full, int sinks, float minus, float& running,
+                                             half8 (&p_hi)[CT][2], half8 (&p_lo)[CT][2])
+{
+    const int g = (threadIdx.x & 63) >> 4;
+    if (scales.x != scales.x || scales.y != scales.y) {         // rows that see some of the block become NaN, the others ignore it
 #pragma unroll
-            for (int j = 0; j < 4; ++j) top = fmaxf(fmaxf(fmaxf(top, s[j][0]), fmaxf(s[j][1], s[j][2])), s[j][3]);
-            top *= scale;
-        } else {
+        for (int t = 0; t < CT; ++t)
+            if (r[t].sees_block(t0, sinks)) r[t].l = __uint_as_float(0x7fc00000u);
+        scales = float2{0.0f, 0.0f};
+    }
+    if (!full) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = t0 + 16 * j + 4 * g + i;
-                    seen[j][i] = t <= position && (t >= low || t < sinks);
-                    s[j][i] *= scale;
-                    top = seen[j][i] ? fmaxf(top, s[j][i]) : top;
-                }
-        }
-        const float next = fmaxf(m, column_max(top)), base = next == -INFINITY ? 0.0f : next;
-        if (keep != 1.0f || __any(next > m)) {
-            const float shrink = __builtin_amdgcn_exp2f(m - base);
-            l *= shrink;
-            const float all = shrink * keep;
+                for (int i = 0; i < 4; ++i)
+                    if (!r[t].sees(t0 + 16 * j + 4 * g + i, sinks)) s[t][j][i] = -INFINITY;
+    }
+    const uint32_t bits = __float_as_uint(scales.y) & 0x7f800000u;
+    const float higher = fmaxf(running, __uint_as_float(bits + 0x00800000u)), keep = running / higher, factor = scales.y * (kPartScale / higher);
+    running = higher;
+    float scale[CT], next[CT], base[CT];
+    bool moved = keep != 1.0f;
 #pragma unroll
-            for (int t = 0; t < DP / 16; ++t) o[t] *= all;
+    for (int t = 0; t < CT; ++t) {
+        // never 0: a hidden score stays at -infinity
+        scale[t] = fmaxf(r[t].c * scales.x, 1e-37f);
+        float top = s[t][0][0];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][j][i]);
+        next[t] = fmaxf(r[t].m, column_max(top) * scale[t]);
+        base[t] = next[t] == -INFINITY ? 0.0f : next[t];
+        moved |= __any(next[t] > r[t].m) != 0;
+    }
+    if (moved) {
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const float shrink = __builtin_amdgcn_exp2f(r[t].m - base[t]), all = shrink * keep;
+            r[t].l *= shrink;
+            r[t].m = next[t];
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) r[t].o[d] *= all;
         }
-        m = next;
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
         float sum = 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             float w[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const int j = 2 * h + u / 4, i = u % 4;
-                float p;
-                if (FULL) {
-                    p = __builtin_amdgcn_exp2f(fmaf(s[j][i], scale, -base));
-                    w[u] = p * factor;
-                } else {
-                    p = seen[j][i] ? __builtin_amdgcn_exp2f(s[j][i] - base) : 0.0f;
-                    w[u] = seen[j][i] ? p * factor : 0.0f;
-                }
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[t][2 * h + u / 4][u % 4], scale[t], -base[t]));
+                w[u] = p * factor;
                 sum += p;
             }
-            split_parts(w, &p_hi[h], &p_lo[h]);
+            split_parts(w, minus, &p_hi[t][h], &p_lo[t][h]);
         }
-        l += sum;
+        r[t].l += sum;
     }
-};
+}
 
 // A block whose every token every row of [first, last] sees.
 __device__ __forceinline__ bool sees_all(const AttendArgs& a, int t0, int first, int last)
 {
     return t0 + kKvBlock - 1 <= first && (a.window == 0 || t0 > last - a.window || t0 + kKvBlock - 1 < a.sinks);
-}
-
-// The running power of two above the value scales of the blocks so far.
-__device__ __forceinline__ float above(float value_scale, float running)
-{
-    const uint32_t bits = __float_as_uint(value_scale);
-    if ((bits & 0x7f800000u) == 0x7f800000u) return running;        // NaN: the probabilities carry it
-    return fmaxf(running, __uint_as_float((bits & 0x7f800000u) + 0x00800000u));
 }
 
 __device__ __forceinline__ void put(float* to, floatx4 v, int d, int width, bool wide)
@@ -356,6 +374,7 @@ __global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_k
 #pragma unroll
     for (int t = 0; t < CT; ++t) r[t].load(a, s, b, kv_head, row0 + t * 16 + (lane & 15));
     float running = kLeastValueScale;
+    const float minus = minus_one();
     while (index < s.end) {
         const int t0 = s.block(index) * kKvBlock;
         floatx4 scores[CT][4];
@@ -364,42 +383,41 @@ __global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_k
 #pragma unroll
             for (int j = 0; j < 4; ++j) scores[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int step = 0; step < DP / 32; ++step)
+        for (int step = 0; step < DP / 32; ++step) {
+            half8 k[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const half8 k = codes.key(step, j);
+            for (int j = 0; j < 4; ++j) k[j] = codes.key(step, j);
 #pragma unroll
-                for (int t = 0; t < CT; ++t) {
-                    scores[t][j] = mma(k, r[t].hi[step], scores[t][j]);
-                    scores[t][j] = mma(k, r[t].lo[step], scores[t][j]);
-                }
-            }
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) scores[t][j] = mma(k[j], r[t].hi[step], scores[t][j]);
+#pragma unroll
+            for (int t = 0; t < CT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) scores[t][j] = mma(k[j], r[t].lo[step], scores[t][j]);
+        }
         const float2 scales = codes.scales;
         index += kWaves;
         const int next = s.block(min(index, s.end - 1));
         if (index < s.end) codes.load_keys(kv, pair, next, lane);
-        const float higher = above(scales.y, running), keep = running / higher, factor = scales.y * (kPartScale / higher);
-        running = higher;
-        const bool full = sees_all(a, t0, s.first, s.last);
         half8 p_hi[CT][2], p_lo[CT][2];
+        softmax_step<DP, CT>(r, scores, scales, t0, sees_all(a, t0, s.first, s.last), a.sinks, minus, running, p_hi, p_lo);
 #pragma unroll
-        for (int t = 0; t < CT; ++t) {
-            if (full)
-                r[t].template softmax<true>(scores[t], t0, a.sinks, scales.x, factor, keep, p_hi[t], p_lo[t]);
-            else
-                r[t].template softmax<false>(scores[t], t0, a.sinks, scales.x, factor, keep, p_hi[t], p_lo[t]);
+        for (int d = 0; d < DP / 16; d += 2) {
+            half8 v[2][2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) v[u][h] = codes.value(d + u, h);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int t = 0; t < CT; ++t) r[t].o[d + u] = mma(v[u][h], part ? p_lo[t][h] : p_hi[t][h], r[t].o[d + u]);
         }
-#pragma unroll
-        for (int d = 0; d < DP / 16; ++d)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const half8 v = codes.value(d, h);
-#pragma unroll
-                for (int t = 0; t < CT; ++t) {
-                    r[t].o[d] = mma(v, p_hi[t][h], r[t].o[d]);
-                    r[t].o[d] = mma(v, p_lo[t][h], r[t].o[d]);
-                }
-            }
         if (index < s.end) codes.load_values(kv, pair, next, lane);
     }
     // the four waves' sums, in a fixed order: 0 + 2 and 1 + 3 through LDS, then the two
@@ -528,6 +546,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_many_kerne
     const int low = a.window > 0 && first >= a.window ? first - a.window + 1 : 0;
     const bool any_row = row_of_wave < s.rows;
     float running = kLeastValueScale;
+    const float minus = minus_one();
     stage(0);
     __syncthreads();
     for (int index = s.begin; index < s.end; ++index) {
@@ -543,38 +562,37 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_many_kerne
 #pragma unroll
                 for (int j = 0; j < 4; ++j) scores[t][j] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int step = 0; step < DP / 32; ++step)
+            for (int step = 0; step < DP / 32; ++step) {
+                half8 x[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const half8 x = __builtin_bit_cast(half8, k[(step * 4 + j) * 64]);
+                for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(half8, k[(step * 4 + j) * 64]);
 #pragma unroll
-                    for (int t = 0; t < CT; ++t) {
-                        scores[t][j] = mma(x, r[t].hi[step], scores[t][j]);
-                        scores[t][j] = mma(x, r[t].lo[step], scores[t][j]);
-                    }
-                }
-            const float higher = above(now.y, running), keep = running / higher, factor = now.y * (kPartScale / higher);
-            running = higher;
-            const bool full = sees_all(a, t0, first, last);
-            half8 p_hi[CT][2], p_lo[CT][2];
+                for (int t = 0; t < CT; ++t)
 #pragma unroll
-            for (int t = 0; t < CT; ++t) {
-                if (full)
-                    r[t].template softmax<true>(scores[t], t0, a.sinks, now.x, factor, keep, p_hi[t], p_lo[t]);
-                else
-                    r[t].template softmax<false>(scores[t], t0, a.sinks, now.x, factor, keep, p_hi[t], p_lo[t]);
+                    for (int j = 0; j < 4; ++j) scores[t][j] = mma(x[j], r[t].hi[step], scores[t][j]);
+#pragma unroll
+                for (int t = 0; t < CT; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) scores[t][j] = mma(x[j], r[t].lo[step], scores[t][j]);
             }
+            half8 p_hi[CT][2], p_lo[CT][2];
+            softmax_step<DP, CT>(r, scores, now, t0, sees_all(a, t0, first, last), a.sinks, minus, running, p_hi, p_lo);
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d)
+            for (int d = 0; d < DP / 16; d += 2) {
+                half8 x[2][2];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const half8 x = __builtin_bit_cast(half8, v[(d * 2 + h) * 64]);
+                for (int u = 0; u < 2; ++u)
 #pragma unroll
-                    for (int t = 0; t < CT; ++t) {
-                        r[t].o[d] = mma(x, p_hi[t][h], r[t].o[d]);
-                        r[t].o[d] = mma(x, p_lo[t][h], r[t].o[d]);
-                    }
-                }
+                    for (int h = 0; h < 2; ++h) x[u][h] = __builtin_bit_cast(half8, v[((d + u) * 2 + h) * 64]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+#pragma unroll
+                            for (int t = 0; t < CT; ++t) r[t].o[d + u] = mma(x[u][h], part ? p_lo[t][h] : p_hi[t][h], r[t].o[d + u]);
+            }
         }
         if (index + 1 < s.end) stage(buffer ^ 1);
         __syncthreads();
