@@ -308,6 +308,16 @@ __device__ void refuse_rows(const AttendArgs& a, const Span& s, int b, int kv_he
     }
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Codes that one workgroup alone reads: streamed past the caches.
+__device__ __forceinline__ uint4 stream(const uint8_t* p)
+{
+    const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));
+    return uint4{x[0], x[1], x[2], x[3]};
+}
+
 template <int DP>
 struct Codes {
     static constexpr int kWhole = DP / 64, kRest = DP % 64 ? 1 : 0;
@@ -319,7 +329,7 @@ struct Codes {
     {
         const uint8_t* at = kv.codes(0, pair, block);
 #pragma unroll
-        for (int u = 0; u < kWhole * 4; ++u) k[u] = *reinterpret_cast<const uint4*>(at + u * 1024 + lane * 16);
+        for (int u = 0; u < kWhole * 4; ++u) k[u] = stream(at + u * 1024 + lane * 16);
         if (kRest) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) rest[j] = *reinterpret_cast<const uint2*>(at + kWhole * 4096 + j * 512 + lane * 8);
@@ -330,7 +340,7 @@ struct Codes {
     {
         const uint8_t* at = kv.codes(1, pair, block);
 #pragma unroll
-        for (int u = 0; u < DP / 16; ++u) v[u] = *reinterpret_cast<const uint4*>(at + u * 1024 + lane * 16);
+        for (int u = 0; u < DP / 16; ++u) v[u] = stream(at + u * 1024 + lane * 16);
     }
     __device__ __forceinline__ half8 key(int step, int j) const
     {
@@ -621,48 +631,65 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_many_kerne
     }
 }
 
-// Adds up the splits of one row: sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k, in the order of the splits within each of the
-// eight groups, then of the groups.
+// Adds up the splits of one row: sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k.  32 lanes hold 128 components, eight groups of
+// them take every eighth split; the groups meet in LDS in their order.  What bounds it is a chain of memory latencies, so
+// the first 64 splits are asked for before it is known how many are in use (those that are not have no weight).
 __global__ __launch_bounds__(kThreads) void attend_join_kernel(const AttendArgs a, int rows_of_tile)
 {
+    constexpr int kAhead = 8;
     __shared__ floatx4 sums[kThreads];
-    __shared__ float tops[kWaves], totals[kWaves];
+    __shared__ float totals[8];
     const KvLayout& kv = a.cache;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, group = tid >> 5;
     const unsigned rows = static_cast<unsigned>(a.tokens) * static_cast<unsigned>(a.group);
     const int row = static_cast<int>(blockIdx.x % rows), pair = static_cast<int>(blockIdx.x / rows);
     const int b = pair / kv.kv_heads, kv_head = pair - b * kv.kv_heads;
-    const Span s = span_of(a, b, row / rows_of_tile * rows_of_tile, rows_of_tile, 0);
-    if (row >= s.rows || s.left_out) return;
-    const int used = splits_used(a, s);
-    if (used == 1) return;
     const size_t from = static_cast<size_t>(blockIdx.x) * a.splits;
-    float m = -INFINITY;
-    for (int k = tid; k < used; k += kThreads) m = fmaxf(m, a.stats[2 * (from + k)]);
-    for (int x = 32; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    if (lane == 0) tops[wave] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    for (int k = tid; k < used; k += kThreads) l += a.stats[2 * (from + k) + 1] * __builtin_amdgcn_exp2f(a.stats[2 * (from + k)] - base);
-    for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
-    if (lane == 0) totals[wave] = l;
-    __syncthreads();
-    l = (totals[0] + totals[1]) + (totals[2] + totals[3]);
-    const int i = row / a.group, h = kv_head * a.group + row % a.group;
-    float* out = a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * kv.head_width;
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + from;
     for (int d0 = 0; d0 < kv.padded; d0 += 128) {
-        const int d = d0 + (tid & 31) * 4;
-        floatx4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (d < kv.padded)
-            for (int k = tid >> 5; k < used; k += 8)
-                x += *reinterpret_cast<const floatx4*>(a.partial + (from + k) * kv.padded + d) * __builtin_amdgcn_exp2f(a.stats[2 * (from + k)] - base);
-        sums[tid] = x;
+        const int d = d0 + (tid & 31) * 4, d_in = min(d, kv.padded - 4);
+        const float* partial = a.partial + from * kv.padded + d_in;
+        floatx4 x[kAhead];
+        float2 st[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int k = min(group + 8 * u, a.splits - 1);
+            x[u] = *reinterpret_cast<const floatx4*>(partial + static_cast<size_t>(k) * kv.padded);
+            st[u] = stats[k];
+        }
+        const Span s = span_of(a, b, row / rows_of_tile * rows_of_tile, rows_of_tile, 0);
+        if (row >= s.rows || s.left_out) return;
+        const int used = splits_used(a, s);
+        if (used == 1) return;
+        float m = -INFINITY;
+        for (int k = tid & 31; k < used; k += 32) m = fmaxf(m, stats[k].x);
+        for (int y = 16; y > 0; y >>= 1) m = fmaxf(m, __shfl_xor(m, y));        // (every half wave finds the same maximum)
+        const float base = m == -INFINITY ? 0.0f : m;
+        floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        float l = 0.0f;
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (group + 8 * u < used) {
+                const float weight = __builtin_amdgcn_exp2f(st[u].x - base);
+                l += st[u].y * weight;
+                sum += x[u] * weight;
+            }
+        for (int k = group + 8 * kAhead; k < used; k += 8) {
+            const float weight = __builtin_amdgcn_exp2f(stats[k].x - base);
+            l += stats[k].y * weight;
+            sum += *reinterpret_cast<const floatx4*>(partial + static_cast<size_t>(k) * kv.padded) * weight;
+        }
+        sums[tid] = sum;
+        if ((tid & 31) == 0) totals[group] = l;
         __syncthreads();
         if (tid < 32 && d < kv.padded) {
-            for (int k = 1; k < 8; ++k) x += sums[tid + 32 * k];
-            put(out, x / l, d, kv.head_width, a.wide);
+            l = totals[0];
+            for (int k = 1; k < 8; ++k) {
+                sum += sums[tid + 32 * k];
+                l += totals[k];
+            }
+            const int i = row / a.group, h = kv_head * a.group + row % a.group;
+            put(a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * kv.head_width, sum / l, d, kv.head_width, a.wide);
         }
         __syncthreads();
     }
@@ -706,7 +733,9 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     }
     p.least = p.few ? kWaves : 8;
     const int64_t groups = static_cast<int64_t>(cache.sequences) * cache.kv_heads * p.row_tiles;
-    int64_t splits = (2 * 2 * static_cast<int64_t>(compute_units) + groups - 1) / groups;
+    // One workgroup a compute unit: every further split costs its prologue and a partial result to add up (one token over
+    // 131000, 8 pairs: 49 us with one a unit, 55 with four, 67 with eight; nothing gained for batches).
+    int64_t splits = (static_cast<int64_t>(compute_units) + groups - 1) / groups;
     const int64_t most = (blocks + p.least - 1) / p.least;
     if (splits > most) splits = most;
     p.splits = static_cast<int>(splits < 1 ? 1 : splits);
