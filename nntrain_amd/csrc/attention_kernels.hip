@@ -300,7 +300,7 @@ __device__ __forceinline__ void put(float* to, floatx4 v, int d, int width, bool
 // Rows of sequences that are left out become NaN.
 __device__ void refuse_rows(const AttendArgs& a, const Span& s, int b, int kv_head, int row0, int rows)
 {
-    for (int e = threadIdx.x; e < rows * a.cache.head_width; e += kThreads) {
+    for (int e = threadIdx.x; e < rows * a.cache.head_width; e += blockDim.x) {
         const int row = row0 + e / a.cache.head_width, d = e % a.cache.head_width;
         if (row >= s.rows) break;
         const int i = row / a.group, h = kv_head * a.group + row % a.group;
@@ -483,12 +483,12 @@ __global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_k
     }
 }
 
-// 128 rows, 32 a wave; blocks staged in LDS as half precision in operand order (every fragment 1 KB in lane order: no bank is
+// CT * 16 rows a wave, W waves; blocks staged in LDS as half precision in operand order (every fragment 1 KB in lane order: no bank is
 // asked twice), two buffers, one barrier a block; the next block's codes travel during the products.
-template <int DP>
-__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void attend_many_kernel(const AttendArgs a)
+template <int DP, int CT, int W>
+__global__ __launch_bounds__(W * 64, 2) void attend_many_kernel(const AttendArgs a)
 {
-    constexpr int CT = 2, kRows = CT * 16 * kWaves, kUnits = DP * kKvBlock / 16, kPerThread = (kUnits + kThreads - 1) / kThreads;
+    constexpr int kThreads = W * 64, kRows = CT * 16 * W, kUnits = DP * kKvBlock / 16, kPerThread = (kUnits + kThreads - 1) / kThreads;
     constexpr int kWhole = DP / 64, kFragments = DP * kKvBlock * 2 / 1024;       // KB of keys (or values) in half precision
     extern __shared__ uint4 staged[];                                            // [2][keys, values][fragment][64]
     const KvLayout& kv = a.cache;
@@ -695,23 +695,33 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(const AttendArgs 
     }
 }
 
+template <int DP, int CT, int W>
+hipError_t launch_many(Lane* lane, const AttendArgs& a, unsigned groups)
+{
+    constexpr int kLds = 2 * 2 * DP * kKvBlock * 2;
+    static LdsLimit limit;
+    const hipError_t e = limit.ensure(lane->device, reinterpret_cast<const void*>(&attend_many_kernel<DP, CT, W>), kLds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((attend_many_kernel<DP, CT, W>), dim3(groups), dim3(W * 64), kLds, lane->stream, a);
+    return hipGetLastError();
+}
+
 template <int DP>
 hipError_t launch(Lane* lane, AttendArgs& a, bool few, int tiles)
 {
     const unsigned groups = static_cast<unsigned>(a.cache.sequences) * static_cast<unsigned>(a.cache.kv_heads) * static_cast<unsigned>(a.row_tiles) * static_cast<unsigned>(a.splits);
     if (few) {
-        if (tiles == 1)
-            hipLaunchKernelGGL((attend_few_kernel<DP, 1>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
-        else
-            hipLaunchKernelGGL((attend_few_kernel<DP, 2>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
+        if constexpr (DP <= 128) {
+            if (tiles == 2) {
+                hipLaunchKernelGGL((attend_few_kernel<DP, 2>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
+                return hipGetLastError();
+            }
+        }
+        hipLaunchKernelGGL((attend_few_kernel<DP, 1>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
         return hipGetLastError();
     }
-    constexpr int kLds = 2 * 2 * DP * kKvBlock * 2;
-    static LdsLimit limit;
-    const hipError_t e = limit.ensure(lane->device, reinterpret_cast<const void*>(&attend_many_kernel<DP>), kLds);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(attend_many_kernel<DP>, dim3(groups), dim3(kThreads), kLds, lane->stream, a);
-    return hipGetLastError();
+    if constexpr (DP <= 128) return tiles == 8 ? launch_many<DP, 2, 4>(lane, a, groups) : launch_many<DP, 1, 4>(lane, a, groups);
+    return launch_many<DP, 1, 8>(lane, a, groups);
 }
 
 }  // namespace
@@ -722,7 +732,13 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     AttendPlan p{};
     const int64_t rows = static_cast<int64_t>(d.tokens) * (d.heads / cache.kv_heads);
     p.few = rows <= 32;
-    p.rows_of_tile = p.few ? (rows <= 16 ? 16 : 32) : 128;
+    const int64_t pairs = static_cast<int64_t>(cache.sequences) * cache.kv_heads;
+    if (p.few)
+        p.rows_of_tile = rows <= 16 || cache.padded > 128 ? 16 : 32;
+    else
+        // 128 rows halve what a row costs in LDS reads and conversions, 64 fill the device twice as well: 1000 tokens of 40 heads
+        // on 8 (320 tiles of 128 rows) take 55 us with 128 and 36 with 64, 2000 tokens 103 either way, 4093 tokens 330 and 361.
+        p.rows_of_tile = cache.padded > 128 || (rows + 127) / 128 * pairs > 2 * compute_units ? 128 : 64;
     p.row_tiles = static_cast<int>((rows + p.rows_of_tile - 1) / p.rows_of_tile);
     // blocks a tile of rows can see at most
     int64_t blocks = cache.blocks;
@@ -732,7 +748,7 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
         blocks = blocks < seen ? blocks : seen;
     }
     p.least = p.few ? kWaves : 8;
-    const int64_t groups = static_cast<int64_t>(cache.sequences) * cache.kv_heads * p.row_tiles;
+    const int64_t groups = pairs * p.row_tiles;
     // One workgroup a compute unit: every further split costs its prologue and a partial result to add up (one token over
     // 131000, 8 pairs: 49 us with one a unit, 55 with four, 67 with eight; nothing gained for batches).
     int64_t splits = (static_cast<int64_t>(compute_units) + groups - 1) / groups;
