@@ -918,9 +918,17 @@ int nnhip_token_log_probs(void* handle, const nnhip_log_probs_desc* d)
     if (!d->log_probs && !d->entropy && !d->top_ids)
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "nothing to compute");
     if (d->rows > 65535) return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "rows %d exceeds 65535", d->rows);
-    const hipError_t e = launch_token_log_probs(lane, *d);
+    const LogProbPlan plan = plan_token_log_probs(*d, lane->compute_units);
+    void* scratch = nullptr;
+    if (plan.scratch_bytes) {
+        const int rc = nnhip_alloc(handle, plan.scratch_bytes, &scratch);
+        if (rc != NNHIP_OK) return rc;
+    }
+    const hipError_t e = launch_token_log_probs(lane, *d, plan, scratch);
+    const int freed = scratch ? nnhip_free(handle, scratch) : NNHIP_OK;
     if (e != hipSuccess) return hip_fail(e, op, lane->device, "log probability launch");
-    lane->counters.kernel_launches += 1;
+    if (freed != NNHIP_OK) return freed;
+    lane->counters.kernel_launches += plan.segments > 1 ? 2 : 1;
     return NNHIP_OK;
 }
 

@@ -173,7 +173,12 @@ struct AttendPlan {
 };
 AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_desc& d, int compute_units);
 hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d, const AttendPlan& plan, float* scratch);
-hipError_t launch_token_log_probs(Lane* lane, const nnhip_log_probs_desc& d);
+struct LogProbPlan {
+    int segments, segment;
+    size_t scratch_bytes;
+};
+LogProbPlan plan_token_log_probs(const nnhip_log_probs_desc& d, int compute_units);
+hipError_t launch_token_log_probs(Lane* lane, const nnhip_log_probs_desc& d, const LogProbPlan& plan, void* scratch);
 // Storage types and widths the bf16 prefill mat-mul covers.
 bool matmul_bf16_supported(uint32_t type, int in_w);
 hipError_t launch_fill_u32(Lane* lane, uint32_t* p, uint32_t value, size_t count);
