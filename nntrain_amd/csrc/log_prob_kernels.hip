@@ -6,11 +6,14 @@
 // probability of a near-certain row consist of.  (T's terms all have one sign: 16 of them meet in FP32, those sums in 64 bits.)
 //
 // Bound by reading the logits once.  A row is cut into segments for as many workgroups as fill the device; a wave takes
-// pieces of 1024 logits of its segment, in rising order, with the next piece on its way, and keeps
-//   - m of the wave, S and T of every lane relative to it (a new maximum is rare: the sums are rescaled then);
-//   - the best logits so far, sorted, one a lane.  Only a piece whose largest logit exceeds the last of them is looked at
-//     again; equal logits keep the order of their indexes because candidates come in rising order and have to be greater.
-// A second launch adds the segments of a row up, if there are several.
+// pieces of 1024 logits of its segment with the next piece on its way, keeps its maximum m, the sums S and T of every lane
+// relative to it (a new maximum is rare: the sums are rescaled then), and writes down each piece's largest logit.
+//
+// The `top` best logits of a row lie in the `top` pieces with the largest maxima (equal maxima by index): any other piece has
+// that many pieces before it, each with a logit that goes before all of its own.  So one workgroup a row picks those pieces and
+// looks at them again, a few KB of the row, with the least of their maxima as the threshold: about as many logits pass as
+// are wanted.  Keeping sorted candidates during the streaming pass instead cost eight times its memory time for 20 of
+// 262144 (92 us for 32 rows).
 #include "nnhip_internal.h"
 
 namespace nnhip {
@@ -18,25 +21,39 @@ namespace nnhip {
 namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
-constexpr int kPiece = 16, kPieceLogits = kPiece * 64;      // logits a lane / a wave has in hand
+constexpr int kHand = 16, kHandLogits = kHand * 64;         // logits a lane / a wave has in hand
+constexpr int kMaxPieces = 512;                             // pieces of a row: 1024 logits each, more in rows above 524288
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLowest = -3.402823466e38f;
 
 struct LogProbArgs {
     nnhip_log_probs_desc d;
-    int segments, segment;      // segments of a row, logits of one (a multiple of kPieceLogits)
+    int segments;               // of a row
+    int64_t segment;            // logits of one (whole pieces)
+    int pieces, piece;          // pieces of a row, logits of one (a multiple of kHandLogits)
     double* sums;               // [row][segment][2]: S, T
     float* tops;                // [row][segment]: m
-    float* values;              // [row][segment][top]
-    int32_t* ids;
+    float* maxima;              // [row][piece]
 };
 
 __device__ __forceinline__ float no_number() { return __uint_as_float(0x7fc00000u); }
 
+// Rotations within 16 lanes, then exchanges of 16 and 32: no LDS.
+template <int CONTROL>
+__device__ __forceinline__ float rotated(float x)
+{
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CONTROL, 0xf, 0xf, false));
+}
 __device__ __forceinline__ float wave_max(float x)
 {
-    for (int y = 32; y > 0; y >>= 1) x = fmaxf(x, __shfl_xor(x, y));
-    return x;
+    x = fmaxf(x, rotated<0x128>(x));
+    x = fmaxf(x, rotated<0x124>(x));
+    x = fmaxf(x, rotated<0x122>(x));
+    x = fmaxf(x, rotated<0x121>(x));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ double wave_sum(double x)
 {
@@ -97,28 +114,26 @@ struct Sums {
     }
 };
 
-// The four waves' results -> thread 0's sums and the `top` best of the workgroup in LDS: every candidate counts those that
-// come before it.
 struct Joined {
     float m[kWaves];
     double S[kWaves], T[kWaves];
+    float maxima[kMaxPieces];
     float value[kWaves * NNHIP_LOG_PROBS_MAX_TOP], best[NNHIP_LOG_PROBS_MAX_TOP];
     int32_t id[kWaves * NNHIP_LOG_PROBS_MAX_TOP], best_id[NNHIP_LOG_PROBS_MAX_TOP];
+    int32_t chosen[NNHIP_LOG_PROBS_MAX_TOP], counts[kMaxPieces / 64];
+    float threshold;
 };
 
-__device__ void join_waves(Joined& j, Sums& sums, const Best& best, int top)
+// The sums of the four waves, in their order; every thread gets them.
+__device__ void join_sums(Joined& j, Sums& sums)
 {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     sums.S = wave_sum(sums.S);
     sums.T = wave_sum(sums.T);
     if (lane == 0) {
         j.m[wave] = sums.m;
         j.S[wave] = sums.S;
         j.T[wave] = sums.T;
-    }
-    if (lane < top) {
-        j.value[wave * top + lane] = best.value;
-        j.id[wave * top + lane] = best.id;
     }
     __syncthreads();
     const float m = fmaxf(fmaxf(j.m[0], j.m[1]), fmaxf(j.m[2], j.m[3]));
@@ -130,7 +145,62 @@ __device__ void join_waves(Joined& j, Sums& sums, const Best& best, int top)
         T += x.T;
     }
     sums = Sums{m, S, T};
-    if (tid < kWaves * top && j.id[tid] >= 0) {
+}
+
+// The `top` best logits of a row whose pieces' maxima are in LDS -> j.best, j.best_id, in their order.
+__device__ void find_best(Joined& j, const LogProbArgs& a, const float* x)
+{
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.d.top, pieces = a.pieces;
+    const int wanted = top < pieces ? top : pieces;
+    if (tid == 0) j.threshold = -INFINITY;                      // (fewer pieces than alternatives: every logit counts)
+    __syncthreads();
+    bool chosen[kMaxPieces / kThreads];
+#pragma unroll
+    for (int r = 0; r < kMaxPieces / kThreads; ++r) {
+        const int p = r * kThreads + tid;
+        chosen[r] = false;
+        if (p < pieces) {                                       // the piece's place among all
+            const float v = j.maxima[p];
+            int before = 0;
+            for (int q = 0; q < pieces; ++q) before += j.maxima[q] > v || (j.maxima[q] == v && q < p) ? 1 : 0;
+            chosen[r] = before < wanted;
+            if (before == wanted - 1 && wanted == top) j.threshold = v;
+        }
+        const uint64_t mask = __ballot(chosen[r]);
+        if (lane == 0) j.counts[r * kWaves + wave] = __popcll(mask);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kMaxPieces / kThreads; ++r) {           // in rising order
+        const uint64_t mask = __ballot(chosen[r]);
+        int at = __popcll(mask & ((1ull << lane) - 1));
+        for (int w = 0; w < r * kWaves + wave; ++w) at += j.counts[w];
+        if (chosen[r]) j.chosen[at] = r * kThreads + tid;
+    }
+    __syncthreads();
+    const float threshold = j.threshold;
+    Best best;
+    best.clear();
+    for (int c = wave; c < wanted; c += kWaves) {
+        const int64_t begin = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(j.chosen[c])) * a.piece;
+        const int64_t end = begin + a.piece < a.d.vocabulary ? begin + a.piece : a.d.vocabulary;
+        for (int64_t at = begin; at < end; at += kHandLogits) {
+            float now[kHand];
+#pragma unroll
+            for (int u = 0; u < kHand; ++u) now[u] = at + u * 64 + lane < end ? x[at + u * 64 + lane] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < kHand; ++u) {
+                const int64_t index = at + u * 64 + lane;
+                best.offer(__ballot(index < end && !(now[u] < threshold) && !(now[u] <= best.last)), now[u], static_cast<int32_t>(index), top);
+            }
+        }
+    }
+    if (lane < top) {
+        j.value[wave * top + lane] = best.value;
+        j.id[wave * top + lane] = best.id;
+    }
+    __syncthreads();
+    if (tid < kWaves * top && j.id[tid] >= 0) {                 // a candidate's place among those of the four waves
         const float v = j.value[tid];
         const int32_t id = j.id[tid];
         int before = 0;
@@ -165,7 +235,6 @@ __device__ void write_row(const nnhip_log_probs_desc& d, int row, const Joined& 
     }
 }
 
-template <bool TOP>
 __global__ __launch_bounds__(kThreads) void log_probs_kernel(const LogProbArgs a)
 {
     __shared__ Joined joined;
@@ -173,75 +242,81 @@ __global__ __launch_bounds__(kThreads) void log_probs_kernel(const LogProbArgs a
     const int row = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.segments)), part = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.segments));
     const float* x = a.d.logits + static_cast<int64_t>(row) * a.d.row_stride;
     const int64_t first = static_cast<int64_t>(part) * a.segment;
-    const int end = static_cast<int>(first + a.segment < a.d.vocabulary ? first + a.segment : a.d.vocabulary);
+    const int64_t end = first + a.segment < a.d.vocabulary ? first + a.segment : a.d.vocabulary;
     Sums sums;
-    Best best;
     sums.clear();
-    best.clear();
-    float now[kPiece], next[kPiece];
-    auto fetch = [&](float (&to)[kPiece], int64_t at) {
-        if (at + kPieceLogits <= end) {
+    float now[kHand], next[kHand];
+    auto fetch = [&](float (&to)[kHand], int64_t at) {
+        const float* from = x + at;
+        if (at + kHandLogits <= end) {
 #pragma unroll
-            for (int u = 0; u < kPiece; ++u) to[u] = __builtin_nontemporal_load(x + at + u * 64 + lane);
+            for (int u = 0; u < kHand; ++u) to[u] = __builtin_nontemporal_load(from + u * 64 + lane);
         } else {
+            const int left = static_cast<int>(end - at);
 #pragma unroll
-            for (int u = 0; u < kPiece; ++u) to[u] = at + u * 64 + lane < end ? x[at + u * 64 + lane] : -INFINITY;
+            for (int u = 0; u < kHand; ++u) to[u] = u * 64 + lane < left ? from[u * 64 + lane] : -INFINITY;
         }
     };
-    int64_t at = first + wave * kPieceLogits;
+    // wave w takes the pieces w, w + 4, ... of the segment
+    const int64_t step = static_cast<int64_t>(kWaves - 1) * a.piece;
+    int64_t at = first + static_cast<int64_t>(wave) * a.piece, piece_end = at + a.piece;
+    float largest = -INFINITY;
     if (at < end) fetch(now, at);
-    for (; at < end; at += kWaves * kPieceLogits) {
-        if (at + kWaves * kPieceLogits < end) fetch(next, at + kWaves * kPieceLogits);
+    while (at < end) {
+        const int64_t following = at + kHandLogits == piece_end ? piece_end + step : at + kHandLogits;
+        if (following < end) fetch(next, following);
         float most = now[0];
 #pragma unroll
-        for (int u = 1; u < kPiece; ++u) most = fmaxf(most, now[u]);
-        if (__any(most > sums.m)) sums.rescale(fmaxf(sums.m, wave_max(most)));
+        for (int u = 1; u < kHand; ++u) most = fmaxf(most, now[u]);
+        most = wave_max(most);
+        if (most > sums.m) sums.rescale(most);
         float t = 0.0f;
 #pragma unroll
-        for (int u = 0; u < kPiece; ++u) {
+        for (int u = 0; u < kHand; ++u) {
             const float d = now[u] - sums.m, e = __builtin_amdgcn_exp2f(d * kLog2e);
             sums.S += static_cast<double>(e);
             t = fmaf(fmaxf(d, -200.0f), e, t);                  // (e is 0 long before: -infinity times 0 must not come up)
         }
         sums.T += static_cast<double>(t);
-        if (TOP && __any(!(most <= best.last) || t != t)) {
-#pragma unroll
-            for (int u = 0; u < kPiece; ++u) {
-                const int64_t index = at + u * 64 + lane;
-                best.offer(__ballot(index < end && !(now[u] <= best.last)), now[u], static_cast<int32_t>(index), a.d.top);
+        if (a.d.top > 0) {
+            largest = __any(t != t) ? INFINITY : fmaxf(largest, most);          // a NaN counts as +infinity
+            if (following != at + kHandLogits || following >= end) {
+                const int piece = static_cast<int>((piece_end - 1) / a.piece);
+                if (lane == 0) {
+                    if (a.segments == 1)
+                        joined.maxima[piece] = largest;
+                    else
+                        a.maxima[static_cast<size_t>(row) * a.pieces + piece] = largest;
+                }
+                largest = -INFINITY;
             }
         }
+        if (following != at + kHandLogits) piece_end = following + a.piece;
+        at = following;
 #pragma unroll
-        for (int u = 0; u < kPiece; ++u) now[u] = next[u];
+        for (int u = 0; u < kHand; ++u) now[u] = next[u];
     }
-    join_waves(joined, sums, best, TOP ? a.d.top : 0);
+    join_sums(joined, sums);
     if (a.segments == 1) {
+        if (a.d.top > 0) find_best(joined, a, x);
         write_row(a.d, row, joined, sums);
-        return;
-    }
-    if (threadIdx.x == 0) {
+    } else if (threadIdx.x == 0) {
         a.tops[blockIdx.x] = sums.m;
         a.sums[2 * static_cast<size_t>(blockIdx.x)] = sums.S;
         a.sums[2 * static_cast<size_t>(blockIdx.x) + 1] = sums.T;
     }
-    if (TOP && static_cast<int>(threadIdx.x) < a.d.top) {
-        const bool there = static_cast<int>(threadIdx.x) < end - first;         // the last segment may hold fewer than `top`
-        const size_t to = static_cast<size_t>(blockIdx.x) * a.d.top + threadIdx.x;
-        a.values[to] = there ? joined.best[threadIdx.x] : 0.0f;
-        a.ids[to] = there ? joined.best_id[threadIdx.x] : -1;
-    }
 }
 
-// The segments of one row: their sums, and their best as candidates in the order of the segments.
+// One row: the sums of its segments, and its best logits.
 __global__ __launch_bounds__(kThreads) void log_probs_join_kernel(const LogProbArgs a)
 {
     __shared__ Joined joined;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x;
     const size_t from = static_cast<size_t>(blockIdx.x) * a.segments;
+    if (a.d.top > 0)
+        for (int p = tid; p < a.pieces; p += kThreads) joined.maxima[p] = a.maxima[static_cast<size_t>(blockIdx.x) * a.pieces + p];
     Sums sums;
-    Best best;
     sums.clear();
-    best.clear();
     float m = kLowest;
     for (int k = tid; k < a.segments; k += kThreads) m = fmaxf(m, a.tops[from + k]);
     sums.m = wave_max(m);
@@ -251,15 +326,8 @@ __global__ __launch_bounds__(kThreads) void log_probs_join_kernel(const LogProbA
         sums.S += x.S;
         sums.T += x.T;
     }
-    const int all = a.segments * a.d.top, each = ((all + kWaves - 1) / kWaves + 63) / 64 * 64;
-    for (int k0 = wave * each; k0 < all && k0 < (wave + 1) * each; k0 += 64) {
-        const int k = k0 + lane;
-        const size_t at = static_cast<size_t>(blockIdx.x) * all + k;
-        const float v = k < all ? a.values[at] : 0.0f;
-        const int32_t id = k < all ? a.ids[at] : -1;
-        best.offer(__ballot(id >= 0 && !(v <= best.last)), v, id, a.d.top);
-    }
-    join_waves(joined, sums, best, a.d.top);
+    join_sums(joined, sums);
+    if (a.d.top > 0) find_best(joined, a, a.d.logits + static_cast<int64_t>(blockIdx.x) * a.d.row_stride);
     write_row(a.d, blockIdx.x, joined, sums);
 }
 
@@ -269,28 +337,29 @@ LogProbPlan plan_token_log_probs(const nnhip_log_probs_desc& d, int compute_unit
 {
     // Eight workgroups of four waves a compute unit, none with less than a piece for each wave where the row allows it.
     LogProbPlan p{};
-    const int64_t pieces = (static_cast<int64_t>(d.vocabulary) + kPieceLogits - 1) / kPieceLogits;
+    const int64_t V = d.vocabulary, hands = (V + kHandLogits - 1) / kHandLogits;
+    const int64_t piece = (hands + kMaxPieces - 1) / kMaxPieces, pieces = (hands + piece - 1) / piece;
     int64_t segments = 8 * static_cast<int64_t>(compute_units) / d.rows;
     if (segments > (pieces + kWaves - 1) / kWaves) segments = (pieces + kWaves - 1) / kWaves;
     if (segments < 1) segments = 1;
     const int64_t each = (pieces + segments - 1) / segments;
-    p.segment = static_cast<int>(each * kPieceLogits < 0x7fffffff ? each * kPieceLogits : 0x7fffffff / kPieceLogits * kPieceLogits);
-    p.segments = static_cast<int>((static_cast<int64_t>(d.vocabulary) + p.segment - 1) / p.segment);
-    if (p.segments > 1) p.scratch_bytes = static_cast<size_t>(d.rows) * p.segments * (16 + 4 + 8 * static_cast<size_t>(d.top));
+    p.piece = static_cast<int>(piece * kHandLogits);
+    p.pieces = static_cast<int>(pieces);
+    p.segments = static_cast<int>((pieces + each - 1) / each);
+    p.segment = each * p.piece;
+    if (p.segments > 1) p.scratch_bytes = static_cast<size_t>(d.rows) * (20 * static_cast<size_t>(p.segments) + 4 * static_cast<size_t>(pieces));
     return p;
 }
 
 hipError_t launch_token_log_probs(Lane* lane, const nnhip_log_probs_desc& d, const LogProbPlan& p, void* scratch)
 {
     const size_t parts = static_cast<size_t>(d.rows) * p.segments;
-    LogProbArgs a{d, p.segments, p.segment, static_cast<double*>(scratch), nullptr, nullptr, nullptr};
-    a.tops = reinterpret_cast<float*>(a.sums + 2 * parts);
-    a.values = a.tops + parts;
-    a.ids = reinterpret_cast<int32_t*>(a.values + parts * d.top);
-    if (d.top > 0)
-        hipLaunchKernelGGL(log_probs_kernel<true>, dim3(static_cast<unsigned>(parts)), dim3(kThreads), 0, lane->stream, a);
-    else
-        hipLaunchKernelGGL(log_probs_kernel<false>, dim3(static_cast<unsigned>(parts)), dim3(kThreads), 0, lane->stream, a);
+    LogProbArgs a{d, p.segments, p.segment, p.pieces, p.piece, static_cast<double*>(scratch), nullptr, nullptr};
+    if (scratch) {
+        a.tops = reinterpret_cast<float*>(a.sums + 2 * parts);
+        a.maxima = a.tops + parts;
+    }
+    hipLaunchKernelGGL(log_probs_kernel, dim3(static_cast<unsigned>(parts)), dim3(kThreads), 0, lane->stream, a);
     if (p.segments > 1) hipLaunchKernelGGL(log_probs_join_kernel, dim3(d.rows), dim3(kThreads), 0, lane->stream, a);
     return hipGetLastError();
 }

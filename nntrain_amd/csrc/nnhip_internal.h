@@ -174,7 +174,8 @@ struct AttendPlan {
 AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_desc& d, int compute_units);
 hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d, const AttendPlan& plan, float* scratch);
 struct LogProbPlan {
-    int segments, segment;
+    int segments, pieces, piece;
+    int64_t segment;
     size_t scratch_bytes;
 };
 LogProbPlan plan_token_log_probs(const nnhip_log_probs_desc& d, int compute_units);
