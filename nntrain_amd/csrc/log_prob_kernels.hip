@@ -33,7 +33,7 @@ struct LogProbArgs {
     int pieces, piece;          // pieces of a row, logits of one (a multiple of kHandLogits)
     double* sums;               // [row][segment][2]: S, T
     float* tops;                // [row][segment]: m
-    float* maxima;              // [row][piece]
+    int32_t* maxima;            // [row][piece], order keys
 };
 
 __device__ __forceinline__ float no_number() { return __uint_as_float(0x7fc00000u); }
@@ -55,10 +55,41 @@ __device__ __forceinline__ float wave_max(float x)
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+template <int CONTROL>
+__device__ __forceinline__ double rotated(double x)
+{
+    const uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    const uint32_t low = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), CONTROL, 0xf, 0xf, false);
+    const uint32_t high = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), CONTROL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(high) << 32 | low);
+}
 __device__ __forceinline__ double wave_sum(double x)
 {
-    for (int y = 32; y > 0; y >>= 1) x += __shfl_xor(x, y);
-    return x;
+    x += rotated<0x128>(x);
+    x += rotated<0x124>(x);
+    x += rotated<0x122>(x);
+    x += rotated<0x121>(x);
+    uint64_t bits = __builtin_bit_cast(uint64_t, x);
+    auto low = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(bits), static_cast<uint32_t>(bits), false, false);
+    auto high = __builtin_amdgcn_permlane16_swap(static_cast<uint32_t>(bits >> 32), static_cast<uint32_t>(bits >> 32), false, false);
+    x = __builtin_bit_cast(double, static_cast<uint64_t>(high[0]) << 32 | low[0]) + __builtin_bit_cast(double, static_cast<uint64_t>(high[1]) << 32 | low[1]);
+    bits = __builtin_bit_cast(uint64_t, x);
+    low = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(bits), static_cast<uint32_t>(bits), false, false);
+    high = __builtin_amdgcn_permlane32_swap(static_cast<uint32_t>(bits >> 32), static_cast<uint32_t>(bits >> 32), false, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(high[0]) << 32 | low[0]) + __builtin_bit_cast(double, static_cast<uint64_t>(high[1]) << 32 | low[1]);
+}
+
+// Integers in the order of the numbers (-0 and +0 the same; a NaN has been replaced by +infinity before).
+__device__ __forceinline__ int32_t order_key(float x)
+{
+    const int32_t bits = static_cast<int32_t>(__float_as_uint(x + 0.0f));
+    return bits ^ ((bits >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float order_value(int32_t key) { return __uint_as_float(static_cast<uint32_t>(key ^ ((key >> 31) & 0x7fffffff))); }
+// One number for the order of candidates: greater logits first, equal ones by index.
+__device__ __forceinline__ uint64_t candidate_key(float x, int32_t id)
+{
+    return static_cast<uint64_t>(static_cast<uint32_t>(order_key(x)) ^ 0x80000000u) << 32 | (0xffffffffu - static_cast<uint32_t>(id));
 }
 
 // The `top` largest logits a wave has seen, sorted, entry i in lane i; empty entries are NaN, which no comparison counts.
@@ -114,116 +145,183 @@ struct Sums {
     }
 };
 
+// What the W waves of a workgroup exchange.
+template <int W>
 struct Joined {
-    float m[kWaves];
-    double S[kWaves], T[kWaves];
-    float maxima[kMaxPieces];
-    float value[kWaves * NNHIP_LOG_PROBS_MAX_TOP], best[NNHIP_LOG_PROBS_MAX_TOP];
-    int32_t id[kWaves * NNHIP_LOG_PROBS_MAX_TOP], best_id[NNHIP_LOG_PROBS_MAX_TOP];
-    int32_t chosen[NNHIP_LOG_PROBS_MAX_TOP], counts[kMaxPieces / 64];
+    float m[W];
+    double S[W], T[W];
+    alignas(16) int32_t maxima[kMaxPieces];                     // order keys
+    float hand[W][kHandLogits];
+    uint64_t candidates[W * NNHIP_LOG_PROBS_MAX_TOP], best[NNHIP_LOG_PROBS_MAX_TOP];
+    int32_t chosen[NNHIP_LOG_PROBS_MAX_TOP], counts[kMaxPieces / 64], found[W];
     float threshold;
 };
 
-// The sums of the four waves, in their order; every thread gets them.
-__device__ void join_sums(Joined& j, Sums& sums)
+// The sums of the waves, in their order; every thread gets them.
+template <int W>
+__device__ void join_sums(Joined<W>& j, Sums& sums)
 {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    sums.S = wave_sum(sums.S);
-    sums.T = wave_sum(sums.T);
+    if (lane == 0) j.m[wave] = sums.m;
+    __syncthreads();
+    float m = j.m[0];
+    for (int w = 1; w < W; ++w) m = fmaxf(m, j.m[w]);
+    sums.rescale(m);                                            // (one exponential a wave, not W in every one)
+    const double S = wave_sum(sums.S), T = wave_sum(sums.T);
     if (lane == 0) {
-        j.m[wave] = sums.m;
-        j.S[wave] = sums.S;
-        j.T[wave] = sums.T;
+        j.S[wave] = S;
+        j.T[wave] = T;
     }
     __syncthreads();
-    const float m = fmaxf(fmaxf(j.m[0], j.m[1]), fmaxf(j.m[2], j.m[3]));
-    double S = 0.0, T = 0.0;
-    for (int w = 0; w < kWaves; ++w) {
-        Sums x{j.m[w], j.S[w], j.T[w]};
-        x.rescale(m);
-        S += x.S;
-        T += x.T;
+    sums.S = sums.T = 0.0;
+    for (int w = 0; w < W; ++w) {
+        sums.S += j.S[w];
+        sums.T += j.T[w];
     }
-    sums = Sums{m, S, T};
+}
+
+// Of the keys in LDS (filled up to `padded` of them, a multiple of 64), those that go before key v of place p: greater ones,
+// and equal ones of lower places.  `low` is the first place of the wave's lanes.
+__device__ __forceinline__ int places_before(const int4* keys, int padded, int32_t v, int p, int low)
+{
+    int before = 0;
+#pragma unroll 8
+    for (int q = 0; q < low / 4; ++q) {
+        const int4 x = keys[q];
+        before += (x.x >= v ? 1 : 0) + (x.y >= v ? 1 : 0) + (x.z >= v ? 1 : 0) + (x.w >= v ? 1 : 0);
+    }
+#pragma unroll 4
+    for (int q = low / 4; q < low / 4 + 16; ++q) {
+        const int4 x = keys[q];
+        before += (x.x > (4 * q < p ? v - 1 : v) ? 1 : 0) + (x.y > (4 * q + 1 < p ? v - 1 : v) ? 1 : 0) + (x.z > (4 * q + 2 < p ? v - 1 : v) ? 1 : 0) +
+                  (x.w > (4 * q + 3 < p ? v - 1 : v) ? 1 : 0);
+    }
+#pragma unroll 8
+    for (int q = low / 4 + 16; q < padded / 4; ++q) {
+        const int4 x = keys[q];
+        before += (x.x > v ? 1 : 0) + (x.y > v ? 1 : 0) + (x.z > v ? 1 : 0) + (x.w > v ? 1 : 0);
+    }
+    return before;
 }
 
 // The `top` best logits of a row whose pieces' maxima are in LDS -> j.best, j.best_id, in their order.
-__device__ void find_best(Joined& j, const LogProbArgs& a, const float* x)
+template <int W>
+__device__ void find_best(Joined<W>& j, const LogProbArgs& a, const float* x)
 {
+    constexpr int kRounds = (kMaxPieces + W * 64 - 1) / (W * 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.d.top, pieces = a.pieces;
     const int wanted = top < pieces ? top : pieces;
+    const int padded = (pieces + 63) / 64 * 64;
     if (tid == 0) j.threshold = -INFINITY;                      // (fewer pieces than alternatives: every logit counts)
+    for (int p = pieces + tid; p < padded; p += W * 64) j.maxima[p] = INT32_MIN;
     __syncthreads();
-    bool chosen[kMaxPieces / kThreads];
+    bool chosen[kRounds];
 #pragma unroll
-    for (int r = 0; r < kMaxPieces / kThreads; ++r) {
-        const int p = r * kThreads + tid;
+    for (int r = 0; r < kRounds; ++r) {
+        const int low = (r * W + wave) * 64, p = low + lane;
         chosen[r] = false;
+        if (low >= pieces) continue;
         if (p < pieces) {                                       // the piece's place among all
-            const float v = j.maxima[p];
-            int before = 0;
-            for (int q = 0; q < pieces; ++q) before += j.maxima[q] > v || (j.maxima[q] == v && q < p) ? 1 : 0;
+            const int32_t v = j.maxima[p];
+            const int before = places_before(reinterpret_cast<const int4*>(j.maxima), padded, v, p, low);
             chosen[r] = before < wanted;
-            if (before == wanted - 1 && wanted == top) j.threshold = v;
+            if (before == wanted - 1 && wanted == top) j.threshold = order_value(v);
         }
         const uint64_t mask = __ballot(chosen[r]);
-        if (lane == 0) j.counts[r * kWaves + wave] = __popcll(mask);
+        if (lane == 0) j.counts[r * W + wave] = __popcll(mask);
     }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kMaxPieces / kThreads; ++r) {           // in rising order
+    for (int r = 0; r < kRounds; ++r) {                         // in rising order
         const uint64_t mask = __ballot(chosen[r]);
+        if (mask == 0) continue;
         int at = __popcll(mask & ((1ull << lane) - 1));
-        for (int w = 0; w < r * kWaves + wave; ++w) at += j.counts[w];
-        if (chosen[r]) j.chosen[at] = r * kThreads + tid;
+        for (int w = 0; w < r * W + wave; ++w) at += j.counts[w];
+        if (chosen[r]) j.chosen[at] = (r * W + wave) * 64 + lane;
     }
     __syncthreads();
     const float threshold = j.threshold;
     Best best;
     best.clear();
-    for (int c = wave; c < wanted; c += kWaves) {
-        const int64_t begin = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(j.chosen[c])) * a.piece;
-        const int64_t end = begin + a.piece < a.d.vocabulary ? begin + a.piece : a.d.vocabulary;
-        for (int64_t at = begin; at < end; at += kHandLogits) {
-            float now[kHand];
+    // piece by piece, 1024 logits at a time, the next ones on their way
+    float now[kHand], next[kHand];
+    int64_t at = 0, end = 0, next_at = 0, next_end = 0;
+    auto fetch = [&](float (&to)[kHand], int64_t from, int64_t until) {
+        const float* y = x + from;
+        const int left = static_cast<int>(until - from < kHandLogits ? until - from : kHandLogits);
 #pragma unroll
-            for (int u = 0; u < kHand; ++u) now[u] = at + u * 64 + lane < end ? x[at + u * 64 + lane] : 0.0f;
-#pragma unroll
-            for (int u = 0; u < kHand; ++u) {
-                const int64_t index = at + u * 64 + lane;
-                best.offer(__ballot(index < end && !(now[u] < threshold) && !(now[u] <= best.last)), now[u], static_cast<int32_t>(index), top);
-            }
+        for (int u = 0; u < kHand; ++u) to[u] = u * 64 + lane < left ? y[u * 64 + lane] : 0.0f;
+    };
+    auto open = [&](int c, int64_t& from, int64_t& until) {
+        from = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(j.chosen[c])) * a.piece;
+        until = from + a.piece < a.d.vocabulary ? from + a.piece : a.d.vocabulary;
+    };
+    int c = wave;
+    if (c < wanted) {
+        open(c, at, end);
+        fetch(now, at, end);
+    }
+    while (c < wanted) {
+        const int left = static_cast<int>(end - at < kHandLogits ? end - at : kHandLogits);
+        next_at = at + kHandLogits;
+        next_end = end;
+        if (next_at >= end) {
+            c += W;
+            if (c < wanted) open(c, next_at, next_end);
         }
+        if (c < wanted) fetch(next, next_at, next_end);
+        // which of the sixteen hold a candidate; those go through LDS, so that the code that takes one in exists once
+        uint32_t some = 0;
+#pragma unroll
+        for (int u = 0; u < kHand; ++u) {
+            some |= __any(u * 64 + lane < left && !(now[u] < threshold)) ? 1u << u : 0u;
+            j.hand[wave][u * 64 + lane] = now[u];
+        }
+        while (some) {
+            const int u = __builtin_ctz(some);
+            some &= some - 1;
+            const float v = j.hand[wave][u * 64 + lane];
+            best.offer(__ballot(u * 64 + lane < left && !(v < threshold) && !(v <= best.last)), v, static_cast<int32_t>(at) + u * 64 + lane, top);
+        }
+        at = next_at;
+        end = next_end;
+#pragma unroll
+        for (int u = 0; u < kHand; ++u) now[u] = next[u];
     }
-    if (lane < top) {
-        j.value[wave * top + lane] = best.value;
-        j.id[wave * top + lane] = best.id;
-    }
+    // the waves' entries side by side, then every entry counts those that go before it
+    const uint64_t held = __ballot(best.id >= 0);
+    if (lane == 0) j.found[wave] = __popcll(held);
     __syncthreads();
-    if (tid < kWaves * top && j.id[tid] >= 0) {                 // a candidate's place among those of the four waves
-        const float v = j.value[tid];
-        const int32_t id = j.id[tid];
+    int place = 0, all = 0;
+    for (int w = 0; w < W; ++w) {
+        place += w < wave ? j.found[w] : 0;
+        all += j.found[w];
+    }
+    if (best.id >= 0) j.candidates[place + lane] = candidate_key(best.value, best.id);          // (entries fill the lanes from 0 on)
+    __syncthreads();
+    for (int e = tid; e < all; e += W * 64) {
+        const uint64_t key = j.candidates[e];
         int before = 0;
-        for (int k = 0; k < kWaves * top; ++k)
-            before += j.id[k] >= 0 && (j.value[k] > v || (j.value[k] == v && j.id[k] < id)) ? 1 : 0;
-        if (before < top) {
-            j.best[before] = v;
-            j.best_id[before] = id;
-        }
+#pragma unroll 4
+        for (int k = 0; k < all; ++k) before += j.candidates[k] > key ? 1 : 0;
+        if (before < top) j.best[before] = key;
     }
     __syncthreads();
 }
 
 // Results of one row from the sums over all of it and the best in LDS.
-__device__ void write_row(const nnhip_log_probs_desc& d, int row, const Joined& j, const Sums& sums)
+template <int W>
+__device__ void write_row(const nnhip_log_probs_desc& d, int row, const Joined<W>& j, const Sums& sums)
 {
     const int tid = threadIdx.x;
     const bool defined = sums.S > 0.0 && sums.S < INFINITY;     // (a NaN or +infinity among the logits makes S NaN)
     const double log_sum = log1p(sums.S - 1.0), m = static_cast<double>(sums.m);
     if (tid < d.top) {
         const size_t at = static_cast<size_t>(row) * d.top + tid;
-        d.top_ids[at] = j.best_id[tid];
-        if (d.top_log_probs) d.top_log_probs[at] = defined ? static_cast<float>((static_cast<double>(j.best[tid]) - m) - log_sum) : no_number();
+        const uint64_t key = j.best[tid];
+        const float x = order_value(static_cast<int32_t>(static_cast<uint32_t>(key >> 32) ^ 0x80000000u));
+        d.top_ids[at] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key));
+        if (d.top_log_probs) d.top_log_probs[at] = defined ? static_cast<float>((static_cast<double>(x) - m) - log_sum) : no_number();
     }
     if (tid == 128 && d.entropy) d.entropy[row] = defined ? static_cast<float>(log_sum - sums.T / sums.S) : no_number();
     if (tid == 64 && d.log_probs) {
@@ -237,7 +335,7 @@ __device__ void write_row(const nnhip_log_probs_desc& d, int row, const Joined& 
 
 __global__ __launch_bounds__(kThreads) void log_probs_kernel(const LogProbArgs a)
 {
-    __shared__ Joined joined;
+    __shared__ Joined<kWaves> joined;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = static_cast<int>(blockIdx.x / static_cast<unsigned>(a.segments)), part = static_cast<int>(blockIdx.x % static_cast<unsigned>(a.segments));
     const float* x = a.d.logits + static_cast<int64_t>(row) * a.d.row_stride;
@@ -284,9 +382,9 @@ __global__ __launch_bounds__(kThreads) void log_probs_kernel(const LogProbArgs a
                 const int piece = static_cast<int>((piece_end - 1) / a.piece);
                 if (lane == 0) {
                     if (a.segments == 1)
-                        joined.maxima[piece] = largest;
+                        joined.maxima[piece] = order_key(largest);
                     else
-                        a.maxima[static_cast<size_t>(row) * a.pieces + piece] = largest;
+                        a.maxima[static_cast<size_t>(row) * a.pieces + piece] = order_key(largest);
                 }
                 largest = -INFINITY;
             }
@@ -308,9 +406,11 @@ __global__ __launch_bounds__(kThreads) void log_probs_kernel(const LogProbArgs a
 }
 
 // One row: the sums of its segments, and its best logits.
-__global__ __launch_bounds__(kThreads) void log_probs_join_kernel(const LogProbArgs a)
+template <int W>
+__global__ __launch_bounds__(W * 64) void log_probs_join_kernel(const LogProbArgs a)
 {
-    __shared__ Joined joined;
+    constexpr int kThreads = W * 64;
+    __shared__ Joined<W> joined;
     const int tid = threadIdx.x;
     const size_t from = static_cast<size_t>(blockIdx.x) * a.segments;
     if (a.d.top > 0)
@@ -357,10 +457,16 @@ hipError_t launch_token_log_probs(Lane* lane, const nnhip_log_probs_desc& d, con
     LogProbArgs a{d, p.segments, p.segment, p.pieces, p.piece, static_cast<double*>(scratch), nullptr, nullptr};
     if (scratch) {
         a.tops = reinterpret_cast<float*>(a.sums + 2 * parts);
-        a.maxima = a.tops + parts;
+        a.maxima = reinterpret_cast<int32_t*>(a.tops + parts);
     }
     hipLaunchKernelGGL(log_probs_kernel, dim3(static_cast<unsigned>(parts)), dim3(kThreads), 0, lane->stream, a);
-    if (p.segments > 1) hipLaunchKernelGGL(log_probs_join_kernel, dim3(d.rows), dim3(kThreads), 0, lane->stream, a);
+    if (p.segments == 1) return hipGetLastError();
+    // Pieces are looked at again by one wave each: sixteen waves a row where that is a row for every compute unit at most
+    // (32 rows, twenty alternatives: WIDEFIG).
+    if (d.rows <= lane->compute_units && d.top > kWaves)
+        hipLaunchKernelGGL(log_probs_join_kernel<16>, dim3(d.rows), dim3(1024), 0, lane->stream, a);
+    else
+        hipLaunchKernelGGL(log_probs_join_kernel<kWaves>, dim3(d.rows), dim3(kThreads), 0, lane->stream, a);
     return hipGetLastError();
 }
 
