@@ -153,7 +153,7 @@ struct Joined {
     alignas(16) int32_t maxima[kMaxPieces];                     // order keys
     float hand[W][kHandLogits];
     uint64_t candidates[W * NNHIP_LOG_PROBS_MAX_TOP], best[NNHIP_LOG_PROBS_MAX_TOP];
-    int32_t chosen[NNHIP_LOG_PROBS_MAX_TOP], counts[kMaxPieces / 64], found[W];
+    int32_t before[kMaxPieces], chosen[NNHIP_LOG_PROBS_MAX_TOP], counts[kMaxPieces / 64], found[W];
     float threshold;
 };
 
@@ -180,26 +180,25 @@ __device__ void join_sums(Joined<W>& j, Sums& sums)
     }
 }
 
-// Of the keys in LDS (filled up to `padded` of them, a multiple of 64), those that go before key v of place p: greater ones,
-// and equal ones of lower places.  `low` is the first place of the wave's lanes.
-__device__ __forceinline__ int places_before(const int4* keys, int padded, int32_t v, int p, int low)
+// Of the 64 keys of group `other` in LDS, those that go before key v of lane `lane` of group `group`: greater ones, and equal
+// ones of lower places.
+__device__ __forceinline__ int places_before(const int4* keys, int other, int32_t v, int group, int lane)
 {
     int before = 0;
+    if (other != group) {
+        const int32_t least = other < group ? v - 1 : v;
 #pragma unroll 8
-    for (int q = 0; q < low / 4; ++q) {
-        const int4 x = keys[q];
-        before += (x.x >= v ? 1 : 0) + (x.y >= v ? 1 : 0) + (x.z >= v ? 1 : 0) + (x.w >= v ? 1 : 0);
+        for (int q = 0; q < 16; ++q) {
+            const int4 x = keys[other * 16 + q];
+            before += (x.x > least ? 1 : 0) + (x.y > least ? 1 : 0) + (x.z > least ? 1 : 0) + (x.w > least ? 1 : 0);
+        }
+        return before;
     }
 #pragma unroll 4
-    for (int q = low / 4; q < low / 4 + 16; ++q) {
-        const int4 x = keys[q];
-        before += (x.x > (4 * q < p ? v - 1 : v) ? 1 : 0) + (x.y > (4 * q + 1 < p ? v - 1 : v) ? 1 : 0) + (x.z > (4 * q + 2 < p ? v - 1 : v) ? 1 : 0) +
-                  (x.w > (4 * q + 3 < p ? v - 1 : v) ? 1 : 0);
-    }
-#pragma unroll 8
-    for (int q = low / 4 + 16; q < padded / 4; ++q) {
-        const int4 x = keys[q];
-        before += (x.x > v ? 1 : 0) + (x.y > v ? 1 : 0) + (x.z > v ? 1 : 0) + (x.w > v ? 1 : 0);
+    for (int q = 0; q < 16; ++q) {
+        const int4 x = keys[other * 16 + q];
+        before += (x.x > (4 * q < lane ? v - 1 : v) ? 1 : 0) + (x.y > (4 * q + 1 < lane ? v - 1 : v) ? 1 : 0) +
+                  (x.z > (4 * q + 2 < lane ? v - 1 : v) ? 1 : 0) + (x.w > (4 * q + 3 < lane ? v - 1 : v) ? 1 : 0);
     }
     return before;
 }
@@ -211,24 +210,27 @@ __device__ void find_best(Joined<W>& j, const LogProbArgs& a, const float* x)
     constexpr int kRounds = (kMaxPieces + W * 64 - 1) / (W * 64);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.d.top, pieces = a.pieces;
     const int wanted = top < pieces ? top : pieces;
-    const int padded = (pieces + 63) / 64 * 64;
+    // The place of every piece among all: groups of 64 pieces against groups of 64, spread over the waves.
+    const int groups = (pieces + 63) / 64;
     if (tid == 0) j.threshold = -INFINITY;                      // (fewer pieces than alternatives: every logit counts)
-    for (int p = pieces + tid; p < padded; p += W * 64) j.maxima[p] = INT32_MIN;
+    for (int p = tid; p < groups * 64; p += W * 64) {
+        j.before[p] = 0;
+        if (p >= pieces) j.maxima[p] = INT32_MIN;
+    }
+    __syncthreads();
+    for (int task = wave; task < groups * groups; task += W) {
+        const int group = task % groups, p = group * 64 + lane;
+        atomicAdd(&j.before[p], places_before(reinterpret_cast<const int4*>(j.maxima), task / groups, j.maxima[p], group, lane));
+    }
     __syncthreads();
     bool chosen[kRounds];
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-        const int low = (r * W + wave) * 64, p = low + lane;
-        chosen[r] = false;
-        if (low >= pieces) continue;
-        if (p < pieces) {                                       // the piece's place among all
-            const int32_t v = j.maxima[p];
-            const int before = places_before(reinterpret_cast<const int4*>(j.maxima), padded, v, p, low);
-            chosen[r] = before < wanted;
-            if (before == wanted - 1 && wanted == top) j.threshold = order_value(v);
-        }
+        const int p = (r * W + wave) * 64 + lane;
+        chosen[r] = p < pieces && j.before[p] < wanted;
+        if (chosen[r] && j.before[p] == wanted - 1 && wanted == top) j.threshold = order_value(j.maxima[p]);
         const uint64_t mask = __ballot(chosen[r]);
-        if (lane == 0) j.counts[r * W + wave] = __popcll(mask);
+        if (lane == 0 && r * W + wave < kMaxPieces / 64) j.counts[r * W + wave] = __popcll(mask);
     }
     __syncthreads();
 #pragma unroll
@@ -417,15 +419,9 @@ __global__ __launch_bounds__(W * 64) void log_probs_join_kernel(const LogProbArg
         for (int p = tid; p < a.pieces; p += kThreads) joined.maxima[p] = a.maxima[static_cast<size_t>(blockIdx.x) * a.pieces + p];
     Sums sums;
     sums.clear();
-    float m = kLowest;
-    for (int k = tid; k < a.segments; k += kThreads) m = fmaxf(m, a.tops[from + k]);
-    sums.m = wave_max(m);
-    for (int k = tid; k < a.segments; k += kThreads) {
-        Sums x{a.tops[from + k], a.sums[2 * (from + k)], a.sums[2 * (from + k) + 1]};
-        x.rescale(sums.m);
-        sums.S += x.S;
-        sums.T += x.T;
-    }
+    // (at most 128 segments: a quarter of the pieces there can be)
+    if (tid < a.segments) sums = Sums{a.tops[from + tid], a.sums[2 * (from + tid)], a.sums[2 * (from + tid) + 1]};
+    sums.rescale(wave_max(sums.m));
     join_sums(joined, sums);
     if (a.d.top > 0) find_best(joined, a, a.d.logits + static_cast<int64_t>(blockIdx.x) * a.d.row_stride);
     write_row(a.d, blockIdx.x, joined, sums);
@@ -461,9 +457,10 @@ hipError_t launch_token_log_probs(Lane* lane, const nnhip_log_probs_desc& d, con
     }
     hipLaunchKernelGGL(log_probs_kernel, dim3(static_cast<unsigned>(parts)), dim3(kThreads), 0, lane->stream, a);
     if (p.segments == 1) return hipGetLastError();
-    // Pieces are looked at again by one wave each: sixteen waves a row where that is a row for every compute unit at most
-    // (32 rows, twenty alternatives: WIDEFIG).
-    if (d.rows <= lane->compute_units && d.top > kWaves)
+    // Pieces are ranked and looked at again wave by wave: sixteen waves a row where the device has room for them and there is
+    // work for them (32 rows of 262144: twenty alternatives 12.7 us with four waves, 10.8 with sixteen, one 8.8 and 8.4; a row of
+    // 32000 and one alternative: 6.1 and 7.5).
+    if (d.rows <= lane->compute_units && d.top > 0 && (p.pieces > 64 || d.top > kWaves))
         hipLaunchKernelGGL(log_probs_join_kernel<16>, dim3(d.rows), dim3(1024), 0, lane->stream, a);
     else
         hipLaunchKernelGGL(log_probs_join_kernel<kWaves>, dim3(d.rows), dim3(kThreads), 0, lane->stream, a);
