@@ -32,7 +32,8 @@ struct StoreArgs {
     int rotary_width;
     uint32_t rotary_style;
     int heads;
-    int slots;              // workgroups of each pair and kind: slot 0 takes the first and the last block, the others one each
+    uint32_t pair_magic;    // 2^32 / (rotary_width / 2), rounded up: e / pairs is the high word of e * pair_magic for e < 2^16
+    int slots;              // workgroups of each pair and kind, a block each
     unsigned kv_groups;     // workgroups of the cache part; the query part follows
     bool wide_k, wide_v;    // rows lie on 16-byte boundaries and head_width is a multiple of 4
     bool wide_q;            // so do those of q and q_out, and the rotary halves are multiples of 4
@@ -113,9 +114,11 @@ __device__ inline void turn(float* a, float* b, double c, double s)
 }
 
 // max |x| over the tile's tokens [from, to) as bits (the order of the numbers, infinity and NaN above all), for every thread.
-__device__ uint32_t largest_of(const float* tile, int pitch, int padded, int from, int to, uint32_t* exchange)
+template <int DP>
+__device__ __forceinline__ uint32_t largest_of(const float* tile, int from, int to, uint32_t* exchange)
 {
-    const int tid = threadIdx.x, quads = padded / 4;
+    constexpr int quads = DP / 4, pitch = DP + 4;
+    const int tid = threadIdx.x;
     uint32_t top = 0;
     for (int e = tid; e < (to - from) * quads; e += kThreads) {
         const int t = from + e / quads;
@@ -136,9 +139,11 @@ __device__ __forceinline__ float scale_of(uint32_t largest)
 }
 
 // New tokens [from, to) of a block into the tile, keys turned by their positions.
-__device__ void load_new(const StoreArgs& a, float* tile, int pitch, int which, int b, int head, int block, int start, int from, int to)
+template <int DP>
+__device__ __forceinline__ void load_new(const StoreArgs& a, float* tile, int which, int b, int head, int block, int start, int from, int to)
 {
-    const int tid = threadIdx.x, width = a.cache.head_width, padded = a.cache.padded, quads = padded / 4;
+    constexpr int padded = DP, quads = DP / 4, pitch = DP + 4;
+    const int tid = threadIdx.x, width = a.cache.head_width;
     const nnhip_rows& rows = which ? a.v : a.k;
     const float* data = rows.data + b * rows.sequence_stride + (static_cast<int64_t>(block) * kKvBlock - start) * rows.token_stride + head * width;
     if (which ? a.wide_v : a.wide_k) {
@@ -160,7 +165,7 @@ __device__ void load_new(const StoreArgs& a, float* tile, int pitch, int which, 
     __syncthreads();
     const int pairs = a.rotary_width / 2;
     for (int e = tid; e < (to - from) * pairs; e += kThreads) {
-        const int t = from + e / pairs, j = e % pairs;
+        const int row = pairs == 1 ? e : static_cast<int>(__umulhi(static_cast<uint32_t>(e), a.pair_magic)), t = from + row, j = e - row * pairs;
         const double2 r = turn_of(block * kKvBlock + t, a.inv_freq[j]);
         int d0, d1;
         rotary_pair(a, j, &d0, &d1);
@@ -169,23 +174,30 @@ __device__ void load_new(const StoreArgs& a, float* tile, int pitch, int which, 
 }
 
 // One block of one head, keys or values: tokens [from, to) of the block are new, those before `from` are there already.
-__device__ void store_block(const StoreArgs& a, float* tile, uint32_t* exchange, int which, int b, int head, int pair, int block, int start,
-                            int from, int to, bool last)
+// `first` is the block that the call begins in.
+template <int DP>
+__device__ __forceinline__ void store_block(const StoreArgs& a, float* tile, uint32_t* exchange, int which, int b, int head, int pair, int block, int first,
+                                            int start, int from, int to, bool last)
 {
+    constexpr int padded = DP, pitch = DP + 4, quads = DP / 4;
     const KvLayout& kv = a.cache;
-    const int tid = threadIdx.x, padded = kv.padded, pitch = padded + 4, quads = padded / 4;
-    float* open = kv.open_values(which, pair);
+    const int tid = threadIdx.x;
     int32_t* marks = kv.marks(which, pair);
     uint8_t* codes = kv.codes(which, pair, block);
     float* scale_at = kv.scales(pair, block) + which;
-    const int held_block = marks[0], held_tokens = marks[1];
+    // The buffer of this block's FP32 values: the one that holds it, else one that does not hold the block the call begins in
+    // (another workgroup may be reading that one; it looks for `first` alone, which this workgroup never writes over).
+    const int2 mark0 = reinterpret_cast<const int2*>(marks)[0], mark1 = reinterpret_cast<const int2*>(marks)[1];
+    const int buffer = mark0.x == block ? 0 : mark1.x == block ? 1 : mark0.x == first ? 1 : 0;
+    const int held_block = buffer ? mark1.x : mark0.x, held_tokens = buffer ? mark1.y : mark0.y;
+    float* open = kv.open_values(which, pair, buffer);
     const float old_scale = from > 0 ? *scale_at : 0.0f;
-    load_new(a, tile, pitch, which, b, head, block, start, from, to);
+    load_new<DP>(a, tile, which, b, head, block, start, from, to);
     __syncthreads();
     bool done = false;
     if (from > 0 && to - from <= kAlone && held_block == block && held_tokens == from) {
         // no new value above the block's largest: the other tokens stay as they are
-        const float scale = scale_of(largest_of(tile, pitch, padded, from, to, exchange));
+        const float scale = scale_of(largest_of<DP>(tile, from, to, exchange));
         if (scale <= old_scale) {
             const Quantizer quantize(old_scale);
             for (int e = tid; e < (to - from) * padded; e += kThreads) {
@@ -214,7 +226,7 @@ __device__ void store_block(const StoreArgs& a, float* tile, uint32_t* exchange,
         for (int e = tid; e < (kKvBlock - to) * quads; e += kThreads)
             *reinterpret_cast<float4*>(&tile[(to + e / quads) * pitch + e % quads * 4]) = float4{0.0f, 0.0f, 0.0f, 0.0f};
         __syncthreads();
-        const float scale = scale_of(largest_of(tile, pitch, padded, 0, to, exchange));
+        const float scale = scale_of(largest_of<DP>(tile, 0, to, exchange));
         if (tid == 0) *scale_at = scale;
         const Quantizer quantize(scale);
         // sixteen codes a thread, in the order of the cache
@@ -256,15 +268,16 @@ __device__ void store_block(const StoreArgs& a, float* tile, uint32_t* exchange,
             *reinterpret_cast<float4*>(&open[t * padded + d]) = *reinterpret_cast<const float4*>(&tile[t * pitch + d]);
         }
         if (tid == 0) {
-            marks[0] = block;
-            marks[1] = to;
+            marks[2 * buffer] = block;
+            marks[2 * buffer + 1] = to;
         }
     }
 }
 
+template <int DP>
 __global__ __launch_bounds__(kThreads) void kv_store_kernel(const StoreArgs a)
 {
-    extern __shared__ float4 shared[];
+    __shared__ float4 shared[kKvBlock * (DP + 4) / 4];
     __shared__ uint32_t exchange[4];
     float* tile = reinterpret_cast<float*>(shared);
     const KvLayout& kv = a.cache;
@@ -279,16 +292,10 @@ __global__ __launch_bounds__(kThreads) void kv_store_kernel(const StoreArgs a)
         const int n = kv_tokens_of(start, kv.capacity, a.tokens, a.counts, b, &left_out);
         if (left_out || n == 0) return;
         const int end = start + n, first = start / kKvBlock, final = (end - 1) / kKvBlock;
-        // The first and the last block go through one workgroup, in this order: the first reads the FP32 values kept of the
-        // open block, the last replaces them.
-        for (int pass = 0; pass < 2; ++pass) {
-            const int block = slot != 0 ? first + slot : pass == 0 ? first : final;
-            if (slot != 0 ? pass == 1 || block >= final : pass == 1 && final == first) break;
-            const int from = block == first ? start - first * kKvBlock : 0;
-            const int to = block == final ? end - final * kKvBlock : kKvBlock;
-            store_block(a, tile, exchange, which, b, head, pair, block, start, from, to, block == final);
-            __syncthreads();
-        }
+        const int block = first + slot;
+        if (block > final) return;
+        const int from = slot == 0 ? start - first * kKvBlock : 0, to = block == final ? end - final * kKvBlock : kKvBlock;
+        store_block<DP>(a, tile, exchange, which, b, head, pair, block, first, start, from, to, block == final);
         return;
     }
     // the query heads of one token: its turns once, in LDS
@@ -422,20 +429,25 @@ static bool on_16_bytes(const nnhip_rows& r)
 
 hipError_t launch_kv_store(Lane* lane, const KvLayout& cache, const nnhip_kv_store_desc& d)
 {
-    StoreArgs a{cache, d.tokens, d.counts, d.k, d.v, d.q, d.q_out, d.inv_freq, d.rotary_width, d.rotary_style, d.heads, 0, 0, false, false, false};
-    // n tokens touch at most (n + 62) / 64 + 1 blocks, of which the first and the last share a workgroup
-    a.slots = static_cast<int>((static_cast<int64_t>(d.tokens) + kKvBlock - 2) / kKvBlock);
-    if (a.slots < 1) a.slots = 1;
+    StoreArgs a{cache, d.tokens, d.counts, d.k, d.v, d.q, d.q_out, d.inv_freq, d.rotary_width, d.rotary_style, d.heads, 0, 0, 0, false, false, false};
+    if (d.rotary_width > 0) {
+        const uint64_t pairs = static_cast<uint64_t>(d.rotary_width) / 2;
+        a.pair_magic = static_cast<uint32_t>(((1ull << 32) + pairs - 1) / pairs);       // (not used for one pair)
+    }
+    a.slots = static_cast<int>((static_cast<int64_t>(d.tokens) + kKvBlock - 2) / kKvBlock + 1);      // the blocks n tokens can touch
     a.kv_groups = static_cast<unsigned>(a.slots) * 2u * static_cast<unsigned>(cache.sequences * cache.kv_heads);
     a.wide_k = cache.head_width % 4 == 0 && on_16_bytes(d.k);
     a.wide_v = cache.head_width % 4 == 0 && on_16_bytes(d.v);
     a.wide_q = cache.head_width % 4 == 0 && d.rotary_width % 8 == 0 && d.rotary_style == NNHIP_ROTARY_HALVES && on_16_bytes(d.q) && on_16_bytes(d.q_out);
-    const unsigned q_groups = d.q.data ? static_cast<unsigned>(cache.sequences) * static_cast<unsigned>(d.tokens) : 0u;
-    const size_t lds = static_cast<size_t>(kKvBlock) * (cache.padded + 4) * sizeof(float);
-    static LdsLimit big;
-    const hipError_t e = big.ensure(lane->device, reinterpret_cast<const void*>(&kv_store_kernel), kKvBlock * (kKvMaxWidth + 4) * 4);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kv_store_kernel, dim3(a.kv_groups + q_groups), dim3(kThreads), lds, lane->stream, a);
+    const dim3 grid(a.kv_groups + (d.q.data ? static_cast<unsigned>(cache.sequences) * static_cast<unsigned>(d.tokens) : 0u)), block(kThreads);
+    switch (cache.padded) {
+    case 32: hipLaunchKernelGGL(kv_store_kernel<32>, grid, block, 0, lane->stream, a); break;
+    case 64: hipLaunchKernelGGL(kv_store_kernel<64>, grid, block, 0, lane->stream, a); break;
+    case 96: hipLaunchKernelGGL(kv_store_kernel<96>, grid, block, 0, lane->stream, a); break;
+    case 128: hipLaunchKernelGGL(kv_store_kernel<128>, grid, block, 0, lane->stream, a); break;
+    case 192: hipLaunchKernelGGL(kv_store_kernel<192>, grid, block, 0, lane->stream, a); break;
+    default: hipLaunchKernelGGL(kv_store_kernel<256>, grid, block, 0, lane->stream, a); break;
+    }
     return hipGetLastError();
 }
 

@@ -66,15 +66,16 @@ struct KvLayout {
     {
         return reinterpret_cast<float*>(base + scales_at) + (static_cast<size_t>(pair) * blocks + block) * 2;
     }
-    // FP32 values of the tokens of the last block stored, [64][padded] (keys turned by their positions)
-    __host__ __device__ float* open_values(int which, int pair) const
+    // FP32 values of the tokens of the last block stored, [64][padded] (keys turned by their positions): two buffers, so that a
+    // call may fill up one block and open another in workgroups that do not wait for each other
+    __host__ __device__ float* open_values(int which, int pair, int buffer) const
     {
-        return reinterpret_cast<float*>(base + open_at) + (static_cast<size_t>(pair) * 2 + which) * kKvBlock * padded;
+        return reinterpret_cast<float*>(base + open_at) + ((static_cast<size_t>(pair) * 2 + which) * 2 + buffer) * kKvBlock * padded;
     }
-    // [2]: that block's index, the number of its tokens that are held
+    // [2 buffers][2]: the index of the block held, the number of its tokens.  No two buffers hold the same block.
     __host__ __device__ int32_t* marks(int which, int pair) const
     {
-        return reinterpret_cast<int32_t*>(base + marks_at) + (static_cast<size_t>(pair) * 2 + which) * 2;
+        return reinterpret_cast<int32_t*>(base + marks_at) + (static_cast<size_t>(pair) * 2 + which) * 4;
     }
 };
 
@@ -91,8 +92,8 @@ inline bool kv_layout(int sequences, int kv_heads, int head_width, int capacity,
     const unsigned __int128 pairs = static_cast<unsigned __int128>(sequences) * kv_heads;
     const unsigned __int128 code = pairs * k.blocks * kKvBlock * k.padded;
     const unsigned __int128 scale = (pairs * k.blocks * 8 + 255) / 256 * 256;
-    const unsigned __int128 open = pairs * 2 * kKvBlock * k.padded * 4;
-    const unsigned __int128 total = 2 * code + scale + open + pairs * 16;
+    const unsigned __int128 open = pairs * 4 * kKvBlock * k.padded * 4;
+    const unsigned __int128 total = 2 * code + scale + open + pairs * 32;
     if (pairs > 0x7fffffff || total >> 62) return false;
     k.code_bytes = static_cast<size_t>(code);
     k.scales_at = static_cast<size_t>(2 * code);

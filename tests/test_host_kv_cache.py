@@ -17,7 +17,7 @@ def _bytes(*args):
 def test_cache_bytes(width, padded):
     sequences, heads, capacity = 3, 5, 130
     pairs, blocks = sequences * heads, 3
-    want = 2 * pairs * blocks * 64 * padded + -(-pairs * blocks * 8 // 256) * 256 + pairs * 2 * 64 * padded * 4 + pairs * 16
+    want = 2 * pairs * blocks * 64 * padded + -(-pairs * blocks * 8 // 256) * 256 + pairs * 4 * 64 * padded * 4 + pairs * 32
     assert _bytes(sequences, heads, width, capacity) == (0, want)
 
 
