@@ -521,12 +521,15 @@ NNHIP_API int nnhip_kv_cache_read(void* lane, const nnhip_kv_cache* cache, const
  * stands at position p = lengths[b] + i and sees key t of head h / (heads / kv_heads) when
  *     t <= p  and  (window == 0  or  t > p - window  or  t < sinks),
  *     out[b, i, h] = sum_t softmax_t(scale * q . K_t) V_t  over the keys it sees (always its own at least).
- * Rows behind counts[b] are not written.  heads is a multiple of kv_heads; scale is finite and >= 0; out must not overlap q.
+ * Rows behind counts[b] are not written.  heads is a multiple of kv_heads; scale is 0 .. 1e30; out must not overlap q.
  * FP32 in and out: queries and probabilities enter the matrix cores as two half-precision parts (22 bits of the largest
  * component of a query row, of the largest probability times value scale), the codes are exact there, all sums and
  * softmax statistics are FP32.  A row that sees a token of a block whose scale is NaN, or whose query holds a NaN or an
- * infinity, is NaN; keys a row does not see have no influence on it.  Results do not depend on the other sequences of the
- * call and are the same on every run.  Scratch memory comes from the lane's kept blocks as in nnhip_quant_matmul.  Replaces the attention core of Qwen35Gpu.AttentionStep
+ * infinity, is NaN; keys a row does not see have no influence on it.  Results are the same on every run.
+ * Scratch memory (partial results of long caches) is one block of the lane that grows with the largest call so far; while a
+ * graph is being captured it cannot grow (NNHIP_ERR_INVALID_ARGUMENT: issue a call at least as large once before), and outgrown
+ * blocks, which a graph may name, are kept until the lane is destroyed.  The graphs of a lane share it with its other work:
+ * replay them with nnhip_graph_launch.  Replaces the attention core of Qwen35Gpu.AttentionStep
  * (Qwen35Gpu.Attention.cs:60-120).  Asynchronous. */
 typedef struct nnhip_attention_desc {
     uint32_t struct_size;
@@ -548,8 +551,9 @@ NNHIP_API int nnhip_cached_attention(void* lane, const nnhip_kv_cache* cache, co
  *                                                          first, equal ones by index; top_log_probs is nullable.
  * One pass over the logits; sums are kept in 64 bits, so that the log probability of a near-certain token and the entropy of
  * a peaked row keep their FP32 accuracy.  A logit of -infinity has probability 0.  A row that holds a NaN or +infinity, or
- * nothing above -infinity, has NaN log probabilities and entropy; in the order of top_ids a NaN counts as +infinity.  Deterministic.  The reference downloads the logits and works on the
- * host (QwenGgufCommand.cs:119-157).  Asynchronous. */
+ * nothing above -infinity, has NaN log probabilities and entropy; in the order of top_ids a NaN counts as +infinity.  Deterministic.
+ * Scratch memory as in nnhip_cached_attention.  The reference downloads the logits and works on the host
+ * (QwenGgufCommand.cs:119-157).  Asynchronous. */
 #define NNHIP_LOG_PROBS_MAX_TOP 64
 typedef struct nnhip_log_probs_desc {
     uint32_t struct_size;

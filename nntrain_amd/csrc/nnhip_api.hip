@@ -300,6 +300,7 @@ int nnhip_lane_destroy(void* handle)
     }
     lane->graphs.clear();
     if (lane->batch_table) (void)hipFree(lane->batch_table);
+    if (lane->scratch) (void)hipFree(lane->scratch);
     for (void* t : lane->retired_tables) (void)hipFree(t);
     for (int i = 0; i < 2; ++i) {
         if (lane->staging[i]) (void)hipHostFree(lane->staging[i]);
@@ -733,6 +734,37 @@ int nnhip_first_token_attention(void* handle, const float* v, float* out, int he
     return NNHIP_OK;
 }
 
+// The lane's scratch block, at least `bytes` large.  It grows to the next power of two from 1 MiB on; an outgrown one is kept
+// until the lane is destroyed.
+static int lane_scratch(uint32_t op, nnhip::Lane* lane, size_t bytes, void** out)
+{
+    using namespace nnhip;
+    if (bytes > lane->scratch_bytes) {
+        if (lane->capturing)
+            return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "scratch memory cannot grow while a graph is being captured: issue a call at least as large once before capturing");
+        size_t capacity = 1u << 20;
+        while (capacity < bytes) capacity <<= 1;
+        void* p = nullptr;
+        hipError_t e = hipMalloc(&p, capacity);
+        if (e == hipErrorOutOfMemory) {
+            (void)hipGetLastError();
+            if (nnhip_lane_trim(lane) == NNHIP_OK) e = hipMalloc(&p, capacity);
+            if (e != hipSuccess) {
+                (void)hipGetLastError();
+                return fail(NNHIP_ERR_OUT_OF_MEMORY, op, lane->device, static_cast<uint32_t>(e), "device allocation of %zu bytes of scratch memory failed", capacity);
+            }
+        }
+        if (e != hipSuccess) return hip_fail(e, op, lane->device, "hipMalloc");
+        std::lock_guard<std::mutex> guard(lane->mutex);
+        ++lane->counters.driver_allocations;
+        if (lane->scratch) lane->retired_tables.push_back(lane->scratch);
+        lane->scratch = p;
+        lane->scratch_bytes = capacity;
+    }
+    *out = lane->scratch;
+    return NNHIP_OK;
+}
+
 // --- 8-bit key/value cache ---------------------------------------------------------------------------------------
 
 // Checks a cache descriptor and derives its layout; `lane` is null for the size query.
@@ -875,26 +907,24 @@ int nnhip_cached_attention(void* handle, const nnhip_kv_cache* cache, const nnhi
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive and heads a positive multiple of kv_heads");
     if (d->window < 0 || d->sinks < 0)
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "window and sinks must not be negative");
-    if (!(d->scale >= 0.0f) || !std::isfinite(d->scale))
-        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "scale must be finite and not negative");
+    if (!(d->scale >= 0.0f) || !(d->scale <= 1e30f))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "scale must be 0 .. 1e30");
     const int64_t width = static_cast<int64_t>(d->heads) * layout.head_width;
     rc = check_rows(op, lane, d->q, layout.sequences, d->tokens, width, false, "q");
     if (rc == NNHIP_OK) rc = check_rows(op, lane, d->out, layout.sequences, d->tokens, width, true, "out");
     if (rc != NNHIP_OK) return rc;
     if (d->q.data == d->out.data) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "out must not overlap q");
-    if (static_cast<__int128>(layout.sequences) * d->tokens * d->heads > 0x7fffffff || width > 0x7fffffff)
+    if (static_cast<__int128>(layout.sequences) * d->tokens * d->heads > 0x3fffffff || width > 0x7fffffff)
         return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, tokens and heads exceed one launch");
-    // partial results of the splits live in a lane block for the duration of the two launches
+    // partial results of the splits live in the lane's scratch memory between the two launches
     const AttendPlan plan = plan_cached_attention(layout, *d, lane->compute_units);
     void* scratch = nullptr;
     if (plan.scratch_floats) {
-        rc = nnhip_alloc(handle, plan.scratch_floats * sizeof(float), &scratch);
+        rc = lane_scratch(op, lane, plan.scratch_floats * sizeof(float), &scratch);
         if (rc != NNHIP_OK) return rc;
     }
     const hipError_t e = launch_cached_attention(lane, layout, *d, plan, static_cast<float*>(scratch));
-    const int freed = scratch ? nnhip_free(handle, scratch) : NNHIP_OK;
     if (e != hipSuccess) return hip_fail(e, op, lane->device, "attention launch");
-    if (freed != NNHIP_OK) return freed;
     lane->counters.kernel_launches += plan.splits > 1 ? 2 : 1;
     return NNHIP_OK;
 }
@@ -921,13 +951,11 @@ int nnhip_token_log_probs(void* handle, const nnhip_log_probs_desc* d)
     const LogProbPlan plan = plan_token_log_probs(*d, lane->compute_units);
     void* scratch = nullptr;
     if (plan.scratch_bytes) {
-        const int rc = nnhip_alloc(handle, plan.scratch_bytes, &scratch);
+        const int rc = lane_scratch(op, lane, plan.scratch_bytes, &scratch);
         if (rc != NNHIP_OK) return rc;
     }
     const hipError_t e = launch_token_log_probs(lane, *d, plan, scratch);
-    const int freed = scratch ? nnhip_free(handle, scratch) : NNHIP_OK;
     if (e != hipSuccess) return hip_fail(e, op, lane->device, "log probability launch");
-    if (freed != NNHIP_OK) return freed;
     lane->counters.kernel_launches += plan.segments > 1 ? 2 : 1;
     return NNHIP_OK;
 }

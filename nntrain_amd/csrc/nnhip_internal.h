@@ -43,7 +43,11 @@ struct Lane {
     std::mutex mutex;                           // guards buffers + counters (uploads may come from loader threads)
     void* batch_table = nullptr;                // device table of the batched mat-vec (written by a kernel on the stream)
     size_t batch_table_bytes = 0;               // its capacity
-    std::vector<void*> retired_tables;          // outgrown tables: freed with the lane, a captured graph may name them
+    std::vector<void*> retired_tables;          // outgrown tables and scratch: freed with the lane, a captured graph may name them
+    // Scratch memory of calls that need some between their own launches (attention over a split cache, log probabilities):
+    // one block for all of them, since the work of a lane and of its graphs runs in the order of its one stream.
+    void* scratch = nullptr;
+    size_t scratch_bytes = 0;
     std::vector<char> batch_shadow;             // the entries the device table holds now (empty: unknown)
     void* static_table = nullptr;               // this device's address of the library's fixed batch workspace
     // Two pinned host buffers (and an event each) through which nnhip_upload_from_file moves a file range: the next piece

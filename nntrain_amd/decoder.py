@@ -10,10 +10,13 @@ output_norm, output) on one lane, either that way (`fused=False`) or with the la
 the residual adds folded into the o and down projections, the value heads read by the o projection itself, SiLU(gate) * up
 left by the stacked gate|up projection): four launches per layer instead of twelve, same bits.
 
-What is NOT here: the attention core and the key/value cache (outside the quantized-linear path).  Every token is
-decoded as the first token of its own sequence, where causal attention is exact without a cache: the single key has
-softmax weight 1, so each query head receives its group's value head (qwen35_gpu.first_token_attention).  All the
-projections of a real decode step run, with their real shapes, which is what the per-token timing is about.
+Without a context (`context_length=0`) every token is decoded as the first token of its own sequence, where causal
+attention is exact without a cache: the single key has softmax weight 1, so each query head receives its group's value
+head (qwen35_gpu.first_token_attention).  All the projections of a real decode step run, with their real shapes, which is
+what the per-token timing is about.  With `context_length=N` the decoder keeps one sequence of up to N tokens: keys and
+values go into an 8-bit cache (kv_cache.QuantizedKvCache) with rotary positions from the file's metadata, and every token
+attends to those before it (six launches per layer in the fused form); `prefill` takes a prompt many rows at a time, `score`
+gives the log probabilities of a text, `reset` starts over.
 
 Timing follows QwenGgufCommand.WriteGeneration (NNtrain.Cli/QwenGgufCommand.cs:119-157): first-token latency and the
 decode rate over the tokens after the first.
@@ -27,6 +30,7 @@ import numpy as np
 
 from . import qwen35_gpu
 from .gguf import GgufReader, InvalidDataError
+from .kv_cache import QuantizedKvCache, Rotary, Rows
 from .lane import HipBuffer, HipExecutionLane
 from .loader import GgufTensorDirectory, HipGgufLoader, NotSupportedError
 from .native import POST_SILU_PAIR
@@ -46,6 +50,12 @@ class DecoderDescriptor:
     head_width: int
     rms_epsilon: float
     vocabulary: int
+    # what attention over a context needs besides (llama.cpp's keys and their defaults)
+    rotary_base: float = 10000.0
+    rotary_width: int = 0           # 0: head_width
+    rotary_pairs: bool = False      # neighbouring components turn together (architecture "llama"), else halves of the head
+    sliding_window: int = 0         # 0: none
+    rotary_scaling: str = "none"
 
     @staticmethod
     def inspect(reader: GgufReader) -> "DecoderDescriptor":
@@ -69,7 +79,10 @@ class DecoderDescriptor:
         if len(token.shape) != 2:
             raise InvalidDataError("GGUF tensor 'token_embd.weight' is not a matrix.")
         d = DecoderDescriptor(arch, need("block_count"), emb, need("feed_forward_length"), heads, kv, head_width,
-                              need("attention.layer_norm_rms_epsilon", float), int(token.shape[1]))
+                              need("attention.layer_norm_rms_epsilon", float), int(token.shape[1]),
+                              float(md.get(f"{arch}.rope.freq_base", 10000.0)), int(md.get(f"{arch}.rope.dimension_count", 0)),
+                              arch == "llama", int(md.get(f"{arch}.attention.sliding_window", 0)),
+                              str(md.get(f"{arch}.rope.scaling.type", "none")))
         if min(d.layer_count, d.embedding_length, d.feed_forward_length, d.head_count, d.kv_head_count, d.head_width) <= 0:
             raise InvalidDataError("GGUF decoder dimensions must be positive.")
         if d.head_count % d.kv_head_count != 0:
@@ -95,28 +108,40 @@ class _Layer:
 class QuantizedDecoder:
     """Weights of one GGUF file resident on one lane, and the per-token loop over them."""
 
-    def __init__(self, lane: HipExecutionLane, reader: GgufReader, fused: bool = True, chunk_bytes: int = 64 << 20):
+    def __init__(self, lane: HipExecutionLane, reader: GgufReader, fused: bool = True, chunk_bytes: int = 64 << 20,
+                 context_length: int = 0, attention_window: int | None = None, attention_sinks: int = 0):
         descriptor = DecoderDescriptor.inspect(reader)
         directory = GgufTensorDirectory(reader)
         loader = HipGgufLoader(lane, reader, chunk_bytes)
         self._build(lane, descriptor, fused,
                     matrix=lambda name, in_w, out_w: loader.load_matrix(directory.matrix(name, in_w, out_w)),
                     dense=lambda name, width: loader.load_dense(directory.dense(name, width)),
-                    has_output="output.weight" in directory, finish=directory.reject_unexpected)
+                    has_output="output.weight" in directory, finish=directory.reject_unexpected,
+                    context=(context_length, attention_window, attention_sinks))
         self.quantized_bytes, self.dense_bytes = loader.quantized_bytes, loader.dense_bytes
 
     @classmethod
     def from_weights(cls, lane: HipExecutionLane, descriptor: DecoderDescriptor, matrix, dense, has_output: bool,
-                     fused: bool = True) -> "QuantizedDecoder":
+                     fused: bool = True, context_length: int = 0, attention_window: int | None = None,
+                     attention_sinks: int = 0) -> "QuantizedDecoder":
         """The same loop over weights that are already on the lane: matrix(name, in_w, out_w) returns a
         HipQuantizedMatrix whose payload is resident, dense(name, width) an FP32 HipBuffer; the decoder owns both."""
         self = cls.__new__(cls)
-        self._build(lane, descriptor, fused, matrix, dense, has_output, finish=lambda: None)
+        self._build(lane, descriptor, fused, matrix, dense, has_output, finish=lambda: None,
+                    context=(context_length, attention_window, attention_sinks))
         self.quantized_bytes = sum(m.storage_bytes for m in self._owned if isinstance(m, HipQuantizedMatrix))
         self.dense_bytes = sum(b.nbytes for b in self._owned if isinstance(b, HipBuffer))
         return self
 
-    def _build(self, lane, descriptor, fused, matrix, dense, has_output, finish) -> None:
+    def _build(self, lane, descriptor, fused, matrix, dense, has_output, finish, context) -> None:
+        self.context_length, window, self.attention_sinks = context
+        self.attention_window = descriptor.sliding_window if window is None else window
+        if self.context_length < 0 or self.attention_window < 0 or self.attention_sinks < 0:
+            raise ValueError("context_length, attention_window and attention_sinks must not be negative.")
+        if self.context_length > 0 and descriptor.rotary_scaling != "none":
+            raise NotSupportedError(f"Rotary scaling '{descriptor.rotary_scaling}' is not supported.")
+        self.cache: QuantizedKvCache | None = None
+        self.position = 0           # tokens of the context so far
         self.lane = lane
         self.fused = fused
         self.descriptor = d = descriptor
@@ -183,8 +208,29 @@ class QuantizedDecoder:
                                        self.logits]
         self._graph = None
         self._graph_start = 0
+        self._prompt: dict[str, HipBuffer] = {}
+        if self.context_length > 0:
+            try:
+                self.cache = own(QuantizedKvCache(lane, d.layer_count, 1, d.kv_head_count, d.head_width, self.context_length))
+                width = d.rotary_width or d.head_width
+                if width > d.head_width or width % 2 != 0 or not d.rotary_base > 0:
+                    raise InvalidDataError("rope.dimension_count must be even and within a head, rope.freq_base positive.")
+                self._rotary = Rotary(own(lane.upload_raw(Rotary.frequencies(width, d.rotary_base))), width, d.rotary_pairs)
+                self._next = own(lane.allocate_bytes(4)), own(lane.allocate(1)), own(lane.allocate(1))
+            except BaseException:
+                self.dispose()
+                raise
 
     # ---------------------------------------------------------------------------------------------- one token
+    def _attend(self, layer: int, q: HipBuffer, k: HipBuffer, v: HipBuffer) -> None:
+        """The attention of one token into _ctx: over the context, or as the first token of a sequence."""
+        d = self.descriptor
+        if self.cache is None:
+            qwen35_gpu.first_token_attention(self.lane, v, d.head_count, d.kv_head_count, d.head_width, out=self._ctx)
+            return
+        self.cache.store(layer, k, v, 1, rotary=self._rotary, q=q, heads=d.head_count)
+        self.cache.attention(layer, q, d.head_count, 1, window=self.attention_window, sinks=self.attention_sinks, out=self._ctx)
+
     def _layers_and_head(self) -> None:
         d, lane = self.descriptor, self.lane
         q_width, kv_width, ffn, eps = d.head_count * d.head_width, d.kv_head_count * d.head_width, d.feed_forward_length, d.rms_epsilon
@@ -192,16 +238,20 @@ class QuantizedDecoder:
         k_view = self._qkv.view(4 * q_width, 4 * kv_width)
         v_view = self._qkv.view(4 * (q_width + kv_width), 4 * kv_width)
         gate_view, up_view = self._gate_up.view(0, 4 * ffn), self._gate_up.view(4 * ffn, 4 * ffn)
-        for L in self.layers:
+        for i, L in enumerate(self.layers):
             cur, nxt = self._hidden[self._cur], self._hidden[self._cur ^ 1]
             if self.fused and L.qkv is not None and L.gate_up is not None:
                 # Four launches.  The o projection reads the value heads itself (what first-token attention would have
                 # copied) and adds the residual stream; the stacked gate | up projection leaves SiLU(gate) * up, so the
                 # down projection reads one vector and nobody forms the product twice.  Every value has the bits of the
-                # one-launch-per-operation sequence.
+                # one-launch-per-operation sequence.  (With a context: the store and the attention in between.)
                 L.qkv.forward_fused(lane, cur, pre_op=PRE_RMS_NORM, norm_weight=L.attn_norm, epsilon=eps, out=self._qkv)
-                L.o.forward_fused(lane, v_view, addend=cur, out=nxt, x_head_width=d.head_width,
-                                  x_head_group=d.head_count // d.kv_head_count)
+                if self.cache is None:
+                    L.o.forward_fused(lane, v_view, addend=cur, out=nxt, x_head_width=d.head_width,
+                                      x_head_group=d.head_count // d.kv_head_count)
+                else:
+                    self._attend(i, q_view, k_view, v_view)
+                    L.o.forward_fused(lane, self._ctx, addend=cur, out=nxt)
                 L.gate_up.forward_fused(lane, nxt, pre_op=PRE_RMS_NORM, norm_weight=L.ffn_norm, epsilon=eps, out=self._act,
                                         post_op=POST_SILU_PAIR)
                 L.down.forward_fused(lane, self._act, addend=nxt, out=nxt)
@@ -213,7 +263,7 @@ class QuantizedDecoder:
                     L.q.forward_fused(lane, cur, pre_op=PRE_RMS_NORM, norm_weight=L.attn_norm, epsilon=eps, x_out=self._norm, out=q_view)
                     L.k.forward(lane, self._norm, None, out=k_view)
                     L.v.forward(lane, self._norm, None, out=v_view)
-                qwen35_gpu.first_token_attention(lane, v_view, d.head_count, d.kv_head_count, d.head_width, out=self._ctx)
+                self._attend(i, q_view, k_view, v_view)
                 L.o.forward(lane, self._ctx, None, out=self._attn)
                 if L.gate_up is not None:
                     L.gate_up.forward_fused(lane, cur, pre_op=PRE_RMS_NORM, x2=self._attn, norm_weight=L.ffn_norm, epsilon=eps,
@@ -229,7 +279,7 @@ class QuantizedDecoder:
                 L.q.forward(lane, self._norm, None, out=q_view)
                 L.k.forward(lane, self._norm, None, out=k_view)
                 L.v.forward(lane, self._norm, None, out=v_view)
-                qwen35_gpu.first_token_attention(lane, v_view, d.head_count, d.kv_head_count, d.head_width, out=self._ctx)
+                self._attend(i, q_view, k_view, v_view)
                 L.o.forward(lane, self._ctx, None, out=self._attn)
                 qwen35_gpu.add_residual_and_rms_norm(lane, cur, self._attn, L.ffn_norm, d.embedding_length, eps, out=self._norm)
                 L.gate.forward(lane, self._norm, None, out=gate_view)
@@ -243,11 +293,15 @@ class QuantizedDecoder:
         else:
             qwen35_gpu.rms_norm(lane, hidden, self.output_norm, 1, d.embedding_length, eps, out=self._norm)
             self.output.forward(lane, self._norm, None, out=self.logits)
+        if self.cache is not None:
+            self.cache.advance(1)
 
     def forward_token(self, token_id: int) -> HipBuffer:
-        """Logits of `token_id` decoded as the first token of a sequence; the buffer is reused by the next call."""
+        """Logits after `token_id`, decoded as the next token of the context (without one: as the first token of a
+        sequence); the buffer is reused by the next call."""
         if not 0 <= token_id < self.descriptor.vocabulary:
             raise IndexError(f"Embedding index {token_id} is outside the vocabulary.")
+        self._room(1)
         if self._graph is not None:
             self._cur = self._graph_start
             self.embedding.dequantize(self.lane, row=token_id, out=self._hidden[self._cur])
@@ -256,7 +310,135 @@ class QuantizedDecoder:
         else:
             self.embedding.dequantize(self.lane, row=token_id, out=self._hidden[self._cur])
             self._layers_and_head()
+        if self.cache is not None:
+            self.position += 1
         return self.logits
+
+    # ---------------------------------------------------------------------------------------------- context
+    def _room(self, tokens: int) -> None:
+        if self.cache is not None and self.position + tokens > self.context_length:
+            raise ValueError(f"The context holds {self.context_length} tokens; {self.position} are in it and {tokens} were to follow.")
+
+    def reset(self) -> None:
+        """Forgets the context."""
+        self._context().reset()
+        self.position = 0
+
+    def _context(self) -> QuantizedKvCache:
+        if self.cache is None:
+            raise ValueError("The decoder has no context: give it a context_length.")
+        return self.cache
+
+    def _prompt_buffers(self, rows: int, head_rows: int) -> dict[str, HipBuffer]:
+        d = self.descriptor
+        q_width, kv_width = d.head_count * d.head_width, d.kv_head_count * d.head_width
+        need = {"hidden": rows * d.embedding_length, "norm": rows * d.embedding_length, "qkv": rows * (q_width + 2 * kv_width),
+                "ctx": rows * q_width, "attn": rows * d.embedding_length, "gate": rows * d.feed_forward_length,
+                "up": rows * d.feed_forward_length, "act": rows * d.feed_forward_length, "logits": head_rows * d.vocabulary,
+                "targets": head_rows, "log_probs": head_rows, "entropy": head_rows}
+        for name, elements in need.items():
+            have = self._prompt.get(name)
+            if elements and (have is None or have.nbytes < 4 * elements):
+                if have is not None:
+                    self._owned.remove(have)
+                    have.dispose()
+                self._prompt[name] = self.lane.allocate(elements)
+                self._owned.append(self._prompt[name])
+        return self._prompt
+
+    def _prompt_layers(self, tokens, buf: dict[str, HipBuffer]) -> None:
+        """The layers over `tokens`, all rows at once; buf["hidden"] receives the last layer's output."""
+        d, lane, n = self.descriptor, self.lane, len(tokens)
+        emb, ffn, eps = d.embedding_length, d.feed_forward_length, d.rms_epsilon
+        q_width, kv_width = d.head_count * d.head_width, d.kv_head_count * d.head_width
+        row = q_width + 2 * kv_width
+        hidden, norm, qkv, ctx, attn = (buf[k] for k in ("hidden", "norm", "qkv", "ctx", "attn"))
+        for i, token in enumerate(tokens):
+            self.embedding.dequantize(lane, row=int(token), out=hidden.view(4 * i * emb, 4 * emb))
+        for i, L in enumerate(self.layers):
+            qwen35_gpu.rms_norm(lane, hidden, L.attn_norm, n, emb, eps, out=norm)
+            if L.qkv is not None:
+                L.qkv.forward(lane, norm, None, rows=n, out=qkv)
+                q, k, v = Rows(qkv, row), Rows(qkv, row, 0, q_width), Rows(qkv, row, 0, q_width + kv_width)
+            else:
+                q, k, v = Rows(qkv, q_width), Rows(qkv, kv_width, 0, n * q_width), Rows(qkv, kv_width, 0, n * (q_width + kv_width))
+                for m, at, width in ((L.q, 0, q_width), (L.k, n * q_width, kv_width), (L.v, n * (q_width + kv_width), kv_width)):
+                    m.forward(lane, norm, None, rows=n, out=qkv.view(4 * at, 4 * n * width))
+            self.cache.store(i, k, v, n, rotary=self._rotary, q=q, heads=d.head_count)
+            self.cache.attention(i, q, d.head_count, n, window=self.attention_window, sinks=self.attention_sinks, out=ctx)
+            L.o.forward(lane, ctx, None, rows=n, out=attn)
+            qwen35_gpu.add_in_place(lane, hidden, attn, n * emb)
+            qwen35_gpu.rms_norm(lane, hidden, L.ffn_norm, n, emb, eps, out=norm)
+            gate, up = (L.gate, L.up) if L.gate_up is None else self._halves(L.gate_up, ffn)
+            gate.forward(lane, norm, None, rows=n, out=buf["gate"])
+            up.forward(lane, norm, None, rows=n, out=buf["up"])
+            qwen35_gpu.silu_multiply(lane, buf["gate"], buf["up"], n * ffn, out=buf["act"])
+            L.down.forward(lane, buf["act"], None, rows=n, out=attn)
+            qwen35_gpu.add_in_place(lane, hidden, attn, n * emb)
+        self.cache.advance(n)
+        self.position += n
+
+    def _halves(self, stacked: HipQuantizedMatrix, rows: int) -> tuple[HipQuantizedMatrix, HipQuantizedMatrix]:
+        """The two projections of a stack, as matrices over windows of its payload."""
+        payload, size = stacked.device_payload(self.lane), stacked.storage_bytes // 2
+        return tuple(HipQuantizedMatrix.from_device(self.lane, payload.view(at, size), stacked.ggml_type, rows, stacked.input_width)
+                     for at in (0, size))
+
+    def _tokens(self, tokens, least: int) -> list[int]:
+        ids = [int(t) for t in tokens]
+        if len(ids) < least:
+            raise ValueError(f"at least {least} token(s) are needed.")
+        if any(not 0 <= t < self.descriptor.vocabulary for t in ids):
+            raise IndexError("A token is outside the vocabulary.")
+        self._context()
+        return ids
+
+    def prefill(self, tokens, rows: int = 512) -> HipBuffer:
+        """Takes `tokens` into the context, `rows` at a time, and returns the logits after the last one (the buffer that
+        forward_token returns)."""
+        ids = self._tokens(tokens, 1)
+        self._room(len(ids))
+        d, lane = self.descriptor, self.lane
+        for at in range(0, len(ids), rows):
+            part = ids[at:at + rows]
+            buf = self._prompt_buffers(len(part), 0)
+            self._prompt_layers(part, buf)
+        last = buf["hidden"].view(4 * (len(part) - 1) * d.embedding_length, 4 * d.embedding_length)
+        qwen35_gpu.rms_norm(lane, last, self.output_norm, 1, d.embedding_length, d.rms_epsilon, out=self._norm)
+        self.output.forward(lane, self._norm, None, out=self.logits)
+        return self.logits
+
+    def score(self, tokens, rows: int = 128) -> tuple[np.ndarray, np.ndarray]:
+        """Natural log probability of every token but the first, given those before it, and the entropy of the distribution
+        it was drawn from; the tokens are taken into the context."""
+        ids = self._tokens(tokens, 2)
+        self._room(len(ids))
+        d, lane = self.descriptor, self.lane
+        log_probs, entropies = [], []
+        for at in range(0, len(ids), rows):
+            part, targets = ids[at:at + rows], ids[at + 1:at + 1 + rows]
+            n = len(targets)
+            buf = self._prompt_buffers(len(part), n)
+            self._prompt_layers(part, buf)
+            if n == 0:
+                break
+            qwen35_gpu.rms_norm(lane, buf["hidden"], self.output_norm, n, d.embedding_length, d.rms_epsilon, out=buf["norm"])
+            self.output.forward(lane, buf["norm"], None, rows=n, out=buf["logits"])
+            lane.write(buf["targets"], np.asarray(targets, np.int32))
+            qwen35_gpu.token_log_probs(lane, buf["logits"], n, d.vocabulary, buf["targets"], out=buf["log_probs"], entropy=buf["entropy"])
+            log_probs.append(lane.read(buf["log_probs"], count=n))
+            entropies.append(lane.read(buf["entropy"], count=n))
+        return np.concatenate(log_probs), np.concatenate(entropies)
+
+    def most_probable(self) -> int:
+        """The token with the largest logit after the last step (the first of equal ones), found on the device."""
+        ids, top, entropy = self._next_buffers()
+        qwen35_gpu.token_log_probs(self.lane, self.logits, 1, self.descriptor.vocabulary, top=1, entropy=entropy, top_ids=ids, top_log_probs=top)
+        return int(self.lane.read(ids, np.int32, 1)[0])
+
+    def _next_buffers(self) -> tuple[HipBuffer, HipBuffer, HipBuffer]:
+        self._context()
+        return self._next
 
     def capture_graph(self) -> None:
         """Records the layers and the head of a token step into a HIP graph that forward_token then replays (the
@@ -272,11 +454,14 @@ class QuantizedDecoder:
         self._graph, self._graph_end = graph, self._cur
 
     # ---------------------------------------------------------------------------------------------- generation
-    def generate(self, first_token: int, max_new_tokens: int, on_token=None) -> tuple[list[int], GenerationTiming]:
-        """Greedy decoding, one token per step (each step sees only its own token: no cache).  The argmax runs on the
-        host over the downloaded logits; first tie wins, as the reference's device ArgMax does."""
+    def generate(self, first_token, max_new_tokens: int, on_token=None) -> tuple[list[int], GenerationTiming]:
+        """Greedy decoding, one token per step; first tie wins, as the reference's device ArgMax does.  With a context
+        `first_token` may be a prompt (a sequence of tokens), every step sees the tokens before it and the argmax runs on the
+        device.  Without one each step sees only its own token and the argmax runs on the host over the downloaded logits."""
         if max_new_tokens < 0:
             raise ValueError("max_new_tokens must not be negative.")
+        if self.cache is not None:
+            return self._generate_in_context(first_token, max_new_tokens, on_token)
         tokens: list[int] = []
         first = last = None
         started = time.perf_counter()
@@ -289,6 +474,26 @@ class QuantizedDecoder:
             tokens.append(token)
             if on_token is not None:
                 on_token(token)
+        total = (time.perf_counter() - started) * 1e3
+        rate = (len(tokens) - 1) * 1000.0 / (last - first) if len(tokens) > 1 and last > first else None
+        return tokens, GenerationTiming(len(tokens), total, first, rate)
+
+    def _generate_in_context(self, prompt, max_new_tokens: int, on_token) -> tuple[list[int], GenerationTiming]:
+        ids = [int(prompt)] if np.ndim(prompt) == 0 else [int(t) for t in prompt]
+        self._room(len(ids) + max(0, max_new_tokens - 1))
+        tokens: list[int] = []
+        first = last = None
+        started = time.perf_counter()
+        for _ in range(max_new_tokens):
+            if tokens or len(ids) == 1:
+                self.forward_token(tokens[-1] if tokens else ids[0])
+            else:
+                self.prefill(ids)
+            tokens.append(self.most_probable())
+            last = (time.perf_counter() - started) * 1e3
+            first = last if first is None else first
+            if on_token is not None:
+                on_token(tokens[-1])
         total = (time.perf_counter() - started) * 1e3
         rate = (len(tokens) - 1) * 1000.0 / (last - first) if len(tokens) > 1 and last > first else None
         return tokens, GenerationTiming(len(tokens), total, first, rate)

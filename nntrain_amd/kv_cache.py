@@ -142,8 +142,8 @@ class QuantizedKvCache:
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative.")
         factor = 1.0 / math.sqrt(self.head_width) if scale is None else scale
-        if not math.isfinite(factor) or factor < 0.0:
-            raise ValueError("scale must be finite and not negative.")
+        if not 0.0 <= factor <= 1e30:
+            raise ValueError("scale must be 0 .. 1e30.")
         width = heads * self.head_width
         rows_in = self._rows(q, tokens, width, "q")
         target = out if out is not None else self.lane.allocate(self.sequences * tokens * width)

@@ -450,6 +450,66 @@ def test_one_captured_step_serves_every_length(lane):
             x.dispose()
 
 
+def test_graphs_and_eager_calls_share_the_scratch_memory():
+    """Long caches leave partial results in the lane's scratch block: two graphs and eager work in turn, two layers each."""
+    kv, heads, width, before = 2, 8, 128, 9000
+    rng = _rng(13)
+    k, v = (_values(rng, 2 * (before + 5), kv, width).reshape(2, 1, before + 5, kv, width) for _ in range(2))
+    with HipExecutionLane(0) as lane, QuantizedKvCache(lane, 2, 1, kv, width, before + 5) as cache:
+        for layer in range(2):
+            _put(lane, cache, layer, k[layer], v[layer])
+        cache.set_lengths([before])
+        qb = [lane.upload_raw(_values(rng, n, heads, width)) for n in (1, 5, 40)]
+        out = [[lane.allocate(n * heads * width) for _ in range(2)] for n in (1, 5, 40)]
+
+        def step(which):
+            n = (1, 5, 40)[which]
+            for layer in range(2):
+                cache.attention(layer, qb[which], heads, min(n, 5), out=out[which][layer])
+
+        def results(which):
+            step_out = [lane.read(b, np.uint32) for b in out[which]]
+            for b in out[which]:
+                lane.fill_u32(b, 0x7FC00000, b.nbytes // 4)
+            return step_out
+
+        # under capture the scratch block cannot come into being
+        lane.graph_begin()
+        cache.advance(1)
+        with pytest.raises(NnHipError, match="before capturing"):
+            step(0)
+        lane.graph_destroy(lane.graph_end())
+        eager = []
+        for which in range(2):
+            step(which)
+            eager.append(results(which))
+        graphs = []
+        for which in range(2):
+            lane.graph_begin()
+            step(which)
+            graphs.append(lane.graph_end())
+        for which in (0, 1, 1, 0, 1, 0):
+            lane.graph_launch(graphs[which])
+            step(1 - which)                                             # eager work behind it, in the same scratch block
+            for w in (which, 1 - which):
+                for a, b in zip(results(w), eager[w]):
+                    assert np.array_equal(a, b)
+        # a larger call grows it; the graphs keep theirs
+        with QuantizedKvCache(lane, 1, 64, 1, 256, 6000) as big:
+            big.set_lengths([5000] * 64)
+            x = lane.allocate(64 * 32 * 256)
+            lane.fill_u32(x, 0, 64 * 32 * 256)
+            big.store(0, x, x, 1)
+            big.attention(0, x, 32, out=lane.allocate(64 * 32 * 256))
+            lane.synchronize()
+        for which in (1, 0):
+            lane.graph_launch(graphs[which])
+            for a, b in zip(results(which), eager[which]):
+                assert np.array_equal(a, b)
+        for g in graphs:
+            lane.graph_destroy(g)
+
+
 def test_refusals(lane):
     with QuantizedKvCache(lane, 1, 2, 2, 64, 100) as cache:
         small, big = lane.allocate(16), lane.allocate(4 * 2 * 4 * 64)
