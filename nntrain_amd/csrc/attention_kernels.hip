@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr float kPartScale = 16384.0f;          // 2^14: probabilities enter the product as p * 2^14
+constexpr float kSlack = 1.9f;                  // the running maximum may lag by this much: 2^1.9 * 2^14 is a half-precision number
 constexpr float kLeastValueScale = 0x1p-100f;   // keeps kPartScale / (running value scale) finite
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -155,7 +156,7 @@ struct Rows16 {
     half8 hi[DP / 32], lo[DP / 32];
     floatx4 o[DP / 16];
     float c;                // what a product of the scaled query and codes is multiplied by, apart from the key scale
-    float m, l;             // running maximum (in powers of two), this lane's part of the sum
+    float m, l;             // running maximum (in powers of two; it may lag by kSlack), this lane's part of the sum
     int position, low;      // of the row; first key of its window
 
     __device__ __forceinline__ void load(const AttendArgs& a, const Span& s, int b, int kv_head, int row)
@@ -248,20 +249,22 @@ __device__ __forceinline__ void softmax_step(Rows16<DP> (&r)[CT], floatx4 (&s)[C
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][j][i]);
-        next[t] = fmaxf(r[t].m, column_max(top) * scale[t]);
-        base[t] = next[t] == -INFINITY ? 0.0f : next[t];
-        moved |= __any(next[t] > r[t].m) != 0;
+        next[t] = column_max(top) * scale[t];
+        moved |= __any(next[t] > r[t].m + kSlack) != 0;
     }
     if (moved) {
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
-            const float shrink = __builtin_amdgcn_exp2f(r[t].m - base[t]), all = shrink * keep;
+            next[t] = fmaxf(r[t].m, next[t]);
+            const float shrink = __builtin_amdgcn_exp2f(r[t].m - (next[t] == -INFINITY ? 0.0f : next[t])), all = shrink * keep;
             r[t].l *= shrink;
             r[t].m = next[t];
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d) r[t].o[d] *= all;
         }
     }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) base[t] = r[t].m == -INFINITY ? 0.0f : r[t].m;
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         float sum = 0.0f;
