@@ -16,12 +16,20 @@ from __future__ import annotations
 
 import ctypes
 import math
-from ctypes import byref, c_uint64, c_void_p
+import struct
+from ctypes import byref, c_uint64
 
 import numpy as np
 
 from .lane import HipBuffer, HipExecutionLane
 from .native import (KV_BLOCK_TOKENS, ROTARY_HALVES, ROTARY_PAIRS, AttentionDesc, KvCacheDesc, KvStoreDesc, RowsDesc, check)
+
+
+# The native descriptors are filled in one go: a token step makes these calls for every layer, and field by field they take
+# longer on the host than the launches on the device.
+_STORE, _ATTENTION, _ROWS = struct.Struct("=Ii Q Qqq Qqq Qqq Qqq Q iIiI"), struct.Struct("=Ii Q Qqq Qqq iiif"), struct.Struct("=Qqq")
+assert _STORE.size == ctypes.sizeof(KvStoreDesc) and _ATTENTION.size == ctypes.sizeof(AttentionDesc)
+_NO_ROWS = (0, 0, 0)
 
 
 class Rows:
@@ -75,6 +83,8 @@ class QuantizedKvCache:
             raise
         self._caches = [KvCacheDesc(ctypes.sizeof(KvCacheDesc), sequences, kv_heads, head_width, capacity, 0, b.ptr, self.lengths.ptr)
                         for b in self._owned[1:]]
+        self._refs = [byref(c) for c in self._caches]
+        self._store, self._attention, self._k_out, self._v_out = KvStoreDesc(), AttentionDesc(), RowsDesc(), RowsDesc()
         self.reset()
 
     # ---- lengths ----
@@ -99,7 +109,7 @@ class QuantizedKvCache:
         """Adds a step's tokens to the lengths, after its last layer."""
         cache = self._cache(0)
         with self.lane.kernel("kv_cache_advance"):
-            check(self.lane._lib.nnhip_kv_cache_advance(self.lane._handle, byref(cache), tokens, self._int32(counts, "counts")),
+            check(self.lane._lib.nnhip_kv_cache_advance(self.lane._handle, cache, tokens, self._int32(counts, "counts") or None),
                   "kv_cache_advance")
 
     # ---- tokens ----
@@ -113,22 +123,25 @@ class QuantizedKvCache:
         if tokens < 1:
             raise ValueError("tokens must be positive.")
         kv_width = self.kv_heads * self.head_width
-        desc = KvStoreDesc(struct_size=ctypes.sizeof(KvStoreDesc), tokens=tokens, counts=self._int32(counts, "counts"),
-                           k=self._rows(k, tokens, kv_width, "k"), v=self._rows(v, tokens, kv_width, "v"))
+        counts_ptr = self._int32(counts, "counts")
+        k_rows, v_rows = self._rows(k, tokens, kv_width, "k"), self._rows(v, tokens, kv_width, "v")
+        turn = (0, 0, 0)
         if rotary is not None:
             if rotary.width > self.head_width:
                 raise ValueError("the rotary width exceeds head_width.")
-            desc.inv_freq, desc.rotary_width, desc.rotary_style = rotary.inv_freq._require(), rotary.width, rotary.style
+            turn = rotary.inv_freq._require(), rotary.width, rotary.style
+        q_rows = out_rows = _NO_ROWS
         if q is not None:
             if rotary is None or heads < 1:
                 raise ValueError("q needs rotary and a positive number of heads.")
-            desc.heads = heads
-            desc.q = self._rows(q, tokens, heads * self.head_width, "q")
-            desc.q_out = desc.q if q_out is None else self._rows(q_out, tokens, heads * self.head_width, "q_out")
+            q_rows = self._rows(q, tokens, heads * self.head_width, "q")
+            out_rows = q_rows if q_out is None else self._rows(q_out, tokens, heads * self.head_width, "q_out")
         elif q_out is not None or heads:
             raise ValueError("q_out and heads need q.")
-        with self.lane.kernel("kv_cache_store"):
-            check(self.lane._lib.nnhip_kv_cache_store(self.lane._handle, byref(cache), byref(desc)), "kv_cache_store")
+        lane = self.lane
+        _STORE.pack_into(self._store, 0, _STORE.size, tokens, counts_ptr, *k_rows, *v_rows, *q_rows, *out_rows, *turn, heads, 0)
+        with lane.kernel("kv_cache_store"):
+            check(lane._lib.nnhip_kv_cache_store(lane._handle, cache, self._store), "kv_cache_store")
 
     def attention(self, layer: int, q: "HipBuffer | Rows", heads: int, tokens: int = 1, *, scale: float | None = None,
                   window: int = 0, sinks: int = 0, counts: HipBuffer | None = None,
@@ -145,13 +158,13 @@ class QuantizedKvCache:
         if not 0.0 <= factor <= 1e30:
             raise ValueError("scale must be 0 .. 1e30.")
         width = heads * self.head_width
-        rows_in = self._rows(q, tokens, width, "q")
-        target = out if out is not None else self.lane.allocate(self.sequences * tokens * width)
+        lane, q_rows, counts_ptr = self.lane, self._rows(q, tokens, width, "q"), self._int32(counts, "counts")
+        target = out if out is not None else lane.allocate(self.sequences * tokens * width)
         try:
-            desc = AttentionDesc(ctypes.sizeof(AttentionDesc), tokens, self._int32(counts, "counts"), rows_in,
-                                 self._rows(target, tokens, width, "out"), heads, min(window, 2**31 - 1), min(sinks, 2**31 - 1), factor)
-            with self.lane.kernel("cached_attention"):
-                check(self.lane._lib.nnhip_cached_attention(self.lane._handle, byref(cache), byref(desc)), "cached_attention")
+            _ATTENTION.pack_into(self._attention, 0, _ATTENTION.size, tokens, counts_ptr, *q_rows, *self._rows(target, tokens, width, "out"),
+                                 heads, min(window, 2**31 - 1), min(sinks, 2**31 - 1), factor)
+            with lane.kernel("cached_attention"):
+                check(lane._lib.nnhip_cached_attention(lane._handle, cache, self._attention), "cached_attention")
         except BaseException:
             if out is None:
                 target.dispose()
@@ -167,28 +180,30 @@ class QuantizedKvCache:
         if k_out is None and v_out is None:
             raise ValueError("read needs k_out or v_out.")
         width = self.kv_heads * self.head_width
-        k = self._rows(k_out, tokens, width, "k_out") if k_out is not None else RowsDesc()
-        v = self._rows(v_out, tokens, width, "v_out") if v_out is not None else RowsDesc()
-        with self.lane.kernel("kv_cache_read"):
-            check(self.lane._lib.nnhip_kv_cache_read(self.lane._handle, byref(cache), self._int32(first, "first"), tokens, byref(k),
-                                                     byref(v)), "kv_cache_read")
+        lane, first_ptr = self.lane, self._int32(first, "first")
+        _ROWS.pack_into(self._k_out, 0, *(self._rows(k_out, tokens, width, "k_out") if k_out is not None else _NO_ROWS))
+        _ROWS.pack_into(self._v_out, 0, *(self._rows(v_out, tokens, width, "v_out") if v_out is not None else _NO_ROWS))
+        with lane.kernel("kv_cache_read"):
+            check(lane._lib.nnhip_kv_cache_read(lane._handle, cache, first_ptr or None, tokens, self._k_out, self._v_out), "kv_cache_read")
 
     # ---- checks ----
-    def _cache(self, layer: int) -> KvCacheDesc:
+    def _cache(self, layer: int):
+        """The native descriptor of a layer's cache, by reference."""
         if not self._owned:
             raise ValueError("the cache has been disposed")
         if not 0 <= layer < self.layers:
             raise IndexError(f"layer {layer} is outside 0 .. {self.layers - 1}.")
-        return self._caches[layer]
+        return self._refs[layer]
 
-    def _int32(self, buffer: HipBuffer | None, name: str) -> c_void_p | None:
+    def _int32(self, buffer: HipBuffer | None, name: str) -> int:
         if buffer is None:
-            return None
+            return 0
         if buffer.nbytes < 4 * self.sequences:
             raise ValueError(f"The buffer '{name}' holds fewer values than there are sequences.")
-        return c_void_p(buffer._require())
+        return buffer._require()
 
-    def _rows(self, rows: "HipBuffer | Rows", tokens: int, width: int, name: str) -> RowsDesc:
+    def _rows(self, rows: "HipBuffer | Rows", tokens: int, width: int, name: str) -> tuple[int, int, int]:
+        """Pointer, token stride and sequence stride of an operand."""
         if rows is None:
             raise TypeError(f"{name} is null.")
         if isinstance(rows, Rows):
@@ -197,7 +212,7 @@ class QuantizedKvCache:
             buffer, token, sequence, offset = rows, width, tokens * width, 0
         if buffer.nbytes < 4 * (offset + (self.sequences - 1) * sequence + (tokens - 1) * token + width):
             raise ValueError(f"The buffer '{name}' is too small for its rows.")
-        return RowsDesc(buffer._require() + 4 * offset, token, sequence)
+        return buffer._require() + 4 * offset, token, sequence
 
     def dispose(self) -> None:
         for b in reversed(self._owned):

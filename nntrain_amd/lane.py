@@ -15,6 +15,9 @@ from . import native
 from .native import check
 
 
+_NO_EVENTS = contextlib.nullcontext()
+
+
 class HipBuffer:
     """Device allocation owned by a lane (the reference's ArcBuffer).  Dispose frees it; the lane frees leaks."""
 
@@ -197,12 +200,14 @@ class HipExecutionLane:
         self._drain_events()
 
     # ---- per-kernel timing (ArcExecutionLane.RecordKernelTime, ArcExecutionLane.cs:727-742) ----
-    @contextlib.contextmanager
     def kernel(self, name: str):
         """Brackets one operation with device events when collect_kernel_events is set (not while a graph is captured)."""
         if not self.collect_kernel_events or self._capturing:
-            yield
-            return
+            return _NO_EVENTS
+        return self._timed_kernel(name)
+
+    @contextlib.contextmanager
+    def _timed_kernel(self, name: str):
         start = self._event_pool.pop() if self._event_pool else HipEvent(self)
         stop = self._event_pool.pop() if self._event_pool else HipEvent(self)
         start.record()

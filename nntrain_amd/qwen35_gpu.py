@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from ctypes import c_void_p
 from typing import NamedTuple
 
@@ -171,6 +172,11 @@ class TokenLogProbs(NamedTuple):
     top_log_probs: HipBuffer | None   # [rows, top] FP32
 
 
+# (one packed write instead of a field at a time: a generation loop makes this call for every token)
+_LOG_PROBS = struct.Struct("=Iiii q QQQQQQ")
+assert _LOG_PROBS.size == ctypes.sizeof(LogProbsDesc)
+
+
 def token_log_probs(lane: HipExecutionLane, logits: HipBuffer, rows: int, vocabulary: int, targets: HipBuffer | None = None,
                     top: int = 0, row_stride: int | None = None, out: HipBuffer | None = None, entropy: HipBuffer | None = None,
                     top_ids: HipBuffer | None = None, top_log_probs: HipBuffer | None = None) -> TokenLogProbs:
@@ -191,24 +197,30 @@ def token_log_probs(lane: HipExecutionLane, logits: HipBuffer, rows: int, vocabu
     _validate_buffer(logits, (rows - 1) * stride + vocabulary, "logits")
     if targets is not None:
         _validate_buffer(targets, rows, "targets")
+    if out is not None:
+        _validate_buffer(out, rows, "out")
+    if entropy is not None:
+        _validate_buffer(entropy, rows, "entropy")
+    if top_ids is not None:
+        _validate_buffer(top_ids, rows * top, "top_ids")
+    if top_log_probs is not None:
+        _validate_buffer(top_log_probs, rows * top, "top_log_probs")
     made: list[HipBuffer] = []
-
-    def output(given: HipBuffer | None, elements: int) -> HipBuffer:
-        buffer = _output(lane, given, elements)
-        if given is None:
-            made.append(buffer)
-        return buffer
-
     try:
-        out = output(out, rows) if targets is not None else None
-        entropy = output(entropy, rows)
-        if top:
-            top_ids, top_log_probs = output(top_ids, rows * top), output(top_log_probs, rows * top)
-        desc = LogProbsDesc(ctypes.sizeof(LogProbsDesc), rows, vocabulary, top, stride, logits._require(),
-                            targets._require() if targets is not None else None, out._require() if out is not None else None,
-                            entropy._require(), top_ids._require() if top else None, top_log_probs._require() if top else None)
+        if out is None and targets is not None:
+            made.append(out := lane.allocate(rows))
+        if entropy is None:
+            made.append(entropy := lane.allocate(rows))
+        if top and top_ids is None:
+            made.append(top_ids := lane.allocate(rows * top))
+        if top and top_log_probs is None:
+            made.append(top_log_probs := lane.allocate(rows * top))
+        desc = LogProbsDesc()
+        _LOG_PROBS.pack_into(desc, 0, _LOG_PROBS.size, rows, vocabulary, top, stride, logits._require(),
+                             targets._require() if targets is not None else 0, out._require() if out is not None else 0,
+                             entropy._require(), top_ids._require() if top else 0, top_log_probs._require() if top else 0)
         with lane.kernel("token_log_probs"):
-            check(lane._lib.nnhip_token_log_probs(lane._handle, ctypes.byref(desc)), "token_log_probs")
+            check(lane._lib.nnhip_token_log_probs(lane._handle, desc), "token_log_probs")
     except BaseException:
         for buffer in made:
             buffer.dispose()
