@@ -178,7 +178,7 @@ struct AttendPlan {
 AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_desc& d, int compute_units);
 hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d, const AttendPlan& plan, float* scratch);
 struct LogProbPlan {
-    int segments, pieces, piece;
+    int segments, pieces, piece, waves;
     int64_t segment;
     size_t scratch_bytes;
 };
