@@ -21,6 +21,8 @@ namespace {
 
 constexpr int kThreads = 256;
 
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
 constexpr int kAlone = 8;       // new tokens that may go in without the rest of their block
 
 struct StoreArgs {
@@ -96,6 +98,25 @@ struct Quantizer {
         }
         return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(n, -127.0f), 127.0f)) + 128);
     }
+    // Sixteen at a time: where every remainder is less than half of scale, the first guesses are the codes (five instructions
+    // a value); otherwise, at a tie or a guess off by one, one by one.
+    __device__ __forceinline__ uint4 operator()(const float (&x)[16]) const
+    {
+        uint32_t word[4] = {0, 0, 0, 0};
+        float worst = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float n = rintf(x[i] * inverse);
+            worst = fmaxf(worst, fabsf(fmaf(-n, scale, x[i])));
+            word[i / 4] = __builtin_amdgcn_cvt_pk_u8_f32(n + 128.0f, i % 4, word[i / 4]);
+        }
+        if (zero || tiny || !(2.0f * worst < scale)) {
+            word[0] = word[1] = word[2] = word[3] = 0;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) word[i / 4] |= (*this)(x[i]) << (8 * (i % 4));
+        }
+        return uint4{word[0], word[1], word[2], word[3]};
+    }
 };
 
 // Components a, b of rotary pair j.
@@ -120,6 +141,7 @@ __device__ __forceinline__ uint32_t largest_of(const float* tile, int from, int 
     constexpr int quads = DP / 4, pitch = DP + 4;
     const int tid = threadIdx.x;
     uint32_t top = 0;
+#pragma unroll 4
     for (int e = tid; e < (to - from) * quads; e += kThreads) {
         const int t = from + e / quads;
         const float4 x = *reinterpret_cast<const float4*>(&tile[t * pitch + e % quads * 4]);
@@ -210,18 +232,29 @@ __device__ __forceinline__ void store_block(const StoreArgs& a, float* tile, uin
     if (!done) {
         // the older tokens: from the FP32 values kept of them, or from their codes where another block has taken the place
         const bool held = held_block == block && held_tokens >= from;
-        for (int e = tid; e < from * quads; e += kThreads) {
-            const int t = e / quads, d = e % quads * 4;
-            float4 x;
-            if (held) {
-                x = *reinterpret_cast<const float4*>(&open[t * padded + d]);
-            } else {
+        if (held) {
+            // (the whole buffer, four loads on their way at a time; what lies behind `from` is not used)
+            const floatx4* kept = reinterpret_cast<const floatx4*>(open) + tid;
+#pragma unroll 1
+            for (int e = tid; e < from * quads; e += 4 * kThreads, kept += 4 * kThreads) {
+                floatx4 x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = e + u * kThreads < kKvBlock * quads ? kept[u * kThreads] : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int at = e + u * kThreads;
+                    if (at < from * quads) *reinterpret_cast<floatx4*>(&tile[at / quads * pitch + at % quads * 4]) = x[u];
+                }
+            }
+        } else {
+            for (int e = tid; e < from * quads; e += kThreads) {
+                const int t = e / quads, d = e % quads * 4;
                 float y[4];
                 for (int u = 0; u < 4; ++u) y[u] = old_scale * static_cast<float>(codes[which ? kv_value_offset(t, d + u) : kv_key_offset(padded, t, d + u)] - 128);
-                x = float4{y[0], y[1], y[2], y[3]};
+                const float4 x = {y[0], y[1], y[2], y[3]};
                 if (last) *reinterpret_cast<float4*>(&open[t * padded + d]) = x;
+                *reinterpret_cast<float4*>(&tile[t * pitch + d]) = x;
             }
-            *reinterpret_cast<float4*>(&tile[t * pitch + d]) = x;
         }
         for (int e = tid; e < (kKvBlock - to) * quads; e += kThreads)
             *reinterpret_cast<float4*>(&tile[(to + e / quads) * pitch + e % quads * 4]) = float4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -231,15 +264,11 @@ __device__ __forceinline__ void store_block(const StoreArgs& a, float* tile, uin
         const Quantizer quantize(scale);
         // sixteen codes a thread, in the order of the cache
         for (int unit = tid; unit < padded * kKvBlock / 16; unit += kThreads) {
-            uint32_t word[4];
+            float x[16];
             if (which) {
                 const int lane = unit & 63, d = (unit >> 6) * 16 + (lane & 15), g = lane >> 4;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    word[j] = 0;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) word[j] |= quantize(tile[(16 * j + 4 * g + i) * pitch + d]) << (8 * i);
-                }
+                for (int i = 0; i < 16; ++i) x[i] = tile[(16 * (i / 4) + 4 * g + i % 4) * pitch + d];
             } else {
                 int t[2], d[2];         // two runs of eight components
                 if (unit < padded / 64 * 256) {
@@ -247,6 +276,7 @@ __device__ __forceinline__ void store_block(const StoreArgs& a, float* tile, uin
                     d[0] = (unit >> 8) * 64 + (unit >> 4 & 3) * 16;
                     d[1] = d[0] + 8;
                 } else {
+#pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int place = 2 * (unit - padded / 64 * 256) + u;
                         t[u] = (place >> 6) * 16 + (place & 15);
@@ -255,11 +285,12 @@ __device__ __forceinline__ void store_block(const StoreArgs& a, float* tile, uin
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float4 x = *reinterpret_cast<const float4*>(&tile[t[j / 2] * pitch + d[j / 2] + j % 2 * 4]);
-                    word[j] = quantize(x.x) | quantize(x.y) << 8 | quantize(x.z) << 16 | quantize(x.w) << 24;
+                    const floatx4 y = *reinterpret_cast<const floatx4*>(&tile[t[j / 2] * pitch + d[j / 2] + j % 2 * 4]);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) x[4 * j + u] = y[u];
                 }
             }
-            reinterpret_cast<uint4*>(codes)[unit] = uint4{word[0], word[1], word[2], word[3]};
+            reinterpret_cast<uint4*>(codes)[unit] = quantize(x);
         }
     }
     if (last) {
