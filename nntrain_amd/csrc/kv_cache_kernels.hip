@@ -7,7 +7,7 @@
 //
 // The rotation is done in 64 bits and rounded once, for positions where an FP32 angle has no correct digit of the turn left:
 // angle = position * inv_freq, reduced by multiples of pi / 2 in two parts, and the Taylor polynomials of degree 17 and 16 on
-// [-pi/4, pi/4], whose remainders are below 2^-58.
+// [-pi/4, pi/4], whose remainders are below 2^-58; in a block every sixteenth token's, the ones between by products.
 //
 // Bound by moving the bytes: a workgroup takes one block of one head, keys or values, through an FP32 tile in LDS from which
 // the codes are read out in the order of the cache (16 bytes a store).  A single token rarely changes its block's scale: then
@@ -185,13 +185,22 @@ __device__ __forceinline__ void load_new(const StoreArgs& a, float* tile, int wh
     }
     if (which || !a.inv_freq) return;
     __syncthreads();
-    const int pairs = a.rotary_width / 2;
-    for (int e = tid; e < (to - from) * pairs; e += kThreads) {
-        const int row = pairs == 1 ? e : static_cast<int>(__umulhi(static_cast<uint32_t>(e), a.pair_magic)), t = from + row, j = e - row * pairs;
-        const double2 r = turn_of(block * kKvBlock + t, a.inv_freq[j]);
-        int d0, d1;
+    // A thread turns one pair of up to sixteen tokens in a row: the first by its angle, each further one by one step more (a
+    // product of complex numbers in 64 bits, 2^-49 off after sixteen).
+    constexpr int kRun = 16;
+    const int pairs = a.rotary_width / 2, runs = (to - from + kRun - 1) / kRun;
+    for (int e = tid; e < runs * pairs; e += kThreads) {
+        const int run = pairs == 1 ? e : static_cast<int>(__umulhi(static_cast<uint32_t>(e), a.pair_magic)), j = e - run * pairs;
+        int t = from + run * kRun, d0, d1;
+        const int end = min(t + kRun, to);
+        const float f = a.inv_freq[j];
+        double2 r = turn_of(block * kKvBlock + t, f);
+        const double2 step = t + 1 < end ? turn_of(1, f) : double2{1.0, 0.0};
         rotary_pair(a, j, &d0, &d1);
-        turn(&tile[t * pitch + d0], &tile[t * pitch + d1], r.x, r.y);
+        for (; t < end; ++t) {
+            turn(&tile[t * pitch + d0], &tile[t * pitch + d1], r.x, r.y);
+            r = double2{fma(r.x, step.x, -r.y * step.y), fma(r.x, step.y, r.y * step.x)};
+        }
     }
 }
 
@@ -380,7 +389,9 @@ __global__ void kv_advance_kernel(int32_t* lengths, const int32_t* counts, int s
     if (!left_out) lengths[b] += n;
 }
 
-// The values of one block of one head, keys or values: codes through LDS, [token][component], FP32 rows out of it.
+// The values of one block of one head, keys or values: codes through LDS, [token][component], so that a wave writes whole rows
+// (32 sequences, 64 tokens of 16 heads of 128: 11.8 us; keys straight from the order of the codes, 16 bytes in each of 16
+// rows a store: 25 us; values straight from it, four components of sixteen tokens a thread: 12.5 us).
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(const KvLayout kv, const int32_t* first, int tokens, int slots, nnhip_rows k, nnhip_rows v,
                                                            bool wide_k, bool wide_v)
 {
