@@ -64,6 +64,14 @@ struct Span {
     __device__ int block(int index) const { return index < sink_blocks ? index : index - sink_blocks + window_block; }
 };
 
+// Up to kTogether blocks are not split: a wave's four blocks take 6 us, a second launch 5.5 (one token, 32 heads on 8 of 128: over
+// 500 tokens 9 us whole and 11.4 split, over 1000 11.8 either way, over 2000 17.4 in two splits and 11.9 in eight).
+constexpr int kTogether = 16;
+__device__ __forceinline__ int blocks_of_split(const AttendArgs& a, int blocks)
+{
+    return blocks <= kTogether ? kTogether : max(a.least, (blocks + a.splits - 1) / a.splits);
+}
+
 // Rows [row0, row0 + rows_of_tile) of a pair, split `split`.  The number of splits in use follows from the blocks there are.
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int row0, int rows_of_tile, int split)
 {
@@ -78,7 +86,7 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int row0, in
     s.window_block = low / kKvBlock;
     s.sink_blocks = min((min(a.sinks, kKvBlock * s.window_block) + kKvBlock - 1) / kKvBlock, s.window_block);
     s.blocks = s.sink_blocks + s.last / kKvBlock + 1 - s.window_block;
-    const int each = max(a.least, (s.blocks + a.splits - 1) / a.splits);
+    const int each = blocks_of_split(a, s.blocks);
     s.begin = static_cast<int>(min(static_cast<int64_t>(split) * each, static_cast<int64_t>(s.blocks)));
     s.end = min(s.begin + each, s.blocks);
     return s;
@@ -86,7 +94,7 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int row0, in
 
 __device__ __forceinline__ int splits_used(const AttendArgs& a, const Span& s)
 {
-    const int each = max(a.least, (s.blocks + a.splits - 1) / a.splits);
+    const int each = blocks_of_split(a, s.blocks);
     return (s.blocks + each - 1) / each;
 }
 
@@ -753,9 +761,11 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     p.least = p.few ? kWaves : 8;
     const int64_t groups = pairs * p.row_tiles;
     // One workgroup a compute unit: every further split costs its prologue and a partial result to add up (one token over
-    // 131000, 8 pairs: 49 us with one a unit, 55 with four, 67 with eight; nothing gained for batches).
-    int64_t splits = (static_cast<int64_t>(compute_units) + groups - 1) / groups;
-    const int64_t most = (blocks + p.least - 1) / p.least;
+    // 131000, 8 pairs: 49 us with one a unit, 55 with four, 67 with eight; nothing gained for batches).  Two where blocks are
+    // small: four sequences of 30000 tokens, 16 heads of 64, take 54 us with one and 46 with two.
+    const int64_t wanted = static_cast<int64_t>(compute_units) * (p.few && cache.padded <= 64 ? 2 : 1);
+    int64_t splits = (wanted + groups - 1) / groups;
+    const int64_t most = blocks <= kTogether ? 1 : (blocks + p.least - 1) / p.least;
     if (splits > most) splits = most;
     p.splits = static_cast<int>(splits < 1 ? 1 : splits);
     if (p.splits > 1) {
