@@ -458,14 +458,14 @@ NNHIP_API int nnhip_lora_b(void* lane, const float* z, const float* b, float* y,
  * the step's tokens after its last layer.  Layers of one model share a lengths array.  A sequence whose length is negative,
  * or whose tokens of this call would pass `capacity`, is left out: nothing of it is stored, and its rows of the attention's
  * output become NaN.  Lengths may be set back (to drop the last tokens, or start over).  Tokens that stay in a block which
- * was not the last one stored count with their 8-bit values when that block is filled up again. */
+ * was not the last one stored may count with their 8-bit values when that block is filled up again. */
 #define NNHIP_KV_BLOCK_TOKENS 64
 typedef struct nnhip_kv_cache {
     uint32_t struct_size;
     int32_t sequences;
     int32_t kv_heads;
     int32_t head_width;
-    int32_t capacity;           /* tokens for each sequence */
+    int32_t capacity;           /* tokens for each sequence, at most 2^30 */
     uint32_t reserved;          /* 0 */
     void* data;
     int32_t* lengths;           /* device, [sequences] */
@@ -525,7 +525,8 @@ NNHIP_API int nnhip_kv_cache_read(void* lane, const nnhip_kv_cache* cache, const
  * FP32 in and out: queries and probabilities enter the matrix cores as two half-precision parts (22 bits of the largest
  * component of a query row, of the largest probability times value scale), the codes are exact there, all sums and
  * softmax statistics are FP32.  A row that sees a token of a block whose scale is NaN, or whose query holds a NaN or an
- * infinity, is NaN; keys a row does not see have no influence on it.  Results are the same on every run.
+ * infinity, is NaN, and so may be one with a score beyond FP32; keys a row does not see have no influence on it.  Results
+ * are the same on every run.
  * Scratch memory (partial results of long caches) is one block of the lane that grows with the largest call so far; while a
  * graph is being captured it cannot grow (NNHIP_ERR_INVALID_ARGUMENT: issue a call at least as large once before), and outgrown
  * blocks, which a graph may name, are kept until the lane is destroyed.  The graphs of a lane share it with its other work:
@@ -549,7 +550,7 @@ NNHIP_API int nnhip_cached_attention(void* lane, const nnhip_kv_cache* cache, co
  *     entropy[r]   = - sum_v p[v] ln p[v]                  (nullable)
  *     top_ids[r, 0..top), top_log_probs[r, 0..top)         the `top` (0 - NNHIP_LOG_PROBS_MAX_TOP) largest logits, largest
  *                                                          first, equal ones by index; top_log_probs is nullable.
- * One pass over the logits; sums are kept in 64 bits, so that the log probability of a near-certain token and the entropy of
+ * rows is at most 65535.  One pass over the logits; sums are kept in 64 bits, so that the log probability of a near-certain token and the entropy of
  * a peaked row keep their FP32 accuracy.  A logit of -infinity has probability 0.  A row that holds a NaN or +infinity, or
  * nothing above -infinity, has NaN log probabilities and entropy; in the order of top_ids a NaN counts as +infinity.  Deterministic.
  * Scratch memory as in nnhip_cached_attention.  The reference downloads the logits and works on the host

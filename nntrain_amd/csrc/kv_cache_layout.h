@@ -94,7 +94,8 @@ inline bool kv_layout(int sequences, int kv_heads, int head_width, int capacity,
     const unsigned __int128 scale = (pairs * k.blocks * 8 + 255) / 256 * 256;
     const unsigned __int128 open = pairs * 4 * kKvBlock * k.padded * 4;
     const unsigned __int128 total = 2 * code + scale + open + pairs * 32;
-    if (pairs > 0x7fffffff || total >> 62) return false;
+    // (positions stay a block away from the largest integer)
+    if (capacity > 0x40000000 || pairs > 0x7fffffff || total >> 62) return false;
     k.code_bytes = static_cast<size_t>(code);
     k.scales_at = static_cast<size_t>(2 * code);
     k.open_at = static_cast<size_t>(2 * code + scale);

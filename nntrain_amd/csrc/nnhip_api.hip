@@ -767,7 +767,9 @@ static int lane_scratch(uint32_t op, nnhip::Lane* lane, size_t bytes, void** out
 
 // --- 8-bit key/value cache ---------------------------------------------------------------------------------------
 
-// Checks a cache descriptor and derives its layout; `lane` is null for the size query.
+static bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; }
+
+// Checks a cache descriptor and derives its layout.
 static int kv_cache_of(uint32_t op, nnhip::Lane* lane, const nnhip_kv_cache* c, nnhip::KvLayout* out)
 {
     using namespace nnhip;
@@ -791,7 +793,7 @@ static int kv_cache_of(uint32_t op, nnhip::Lane* lane, const nnhip_kv_cache* c, 
 static int check_rows(uint32_t op, nnhip::Lane* lane, const nnhip_rows& r, int sequences, int tokens, int64_t width, bool output, const char* name)
 {
     using namespace nnhip;
-    if (!r.data || (reinterpret_cast<uintptr_t>(r.data) & 3u))
+    if (!r.data || misaligned(r.data))
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "%s is null or not 4-byte aligned", name);
     if (r.token_stride < 0 || r.sequence_stride < 0)
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "the strides of %s must not be negative", name);
@@ -824,7 +826,8 @@ int nnhip_kv_cache_store(void* handle, const nnhip_kv_cache* cache, const nnhip_
     if (rc != NNHIP_OK) return rc;
     if (!d || d->struct_size != sizeof(nnhip_kv_store_desc) || d->reserved != 0)
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "descriptor is null, has the wrong struct_size or a reserved field that is not 0");
-    if (d->tokens < 1) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive");
+    if (d->tokens < 1 || misaligned(d->counts) || misaligned(d->inv_freq))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive, counts and inv_freq 4-byte aligned");
     if (d->inv_freq) {
         if (d->rotary_width < 2 || d->rotary_width % 2 != 0 || d->rotary_width > layout.head_width || d->rotary_style > NNHIP_ROTARY_PAIRS)
             return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "rotary_width must be even and within the head, rotary_style a known one");
@@ -863,7 +866,7 @@ int nnhip_kv_cache_advance(void* handle, const nnhip_kv_cache* cache, int tokens
     KvLayout layout;
     const int rc = kv_cache_of(op, lane, cache, &layout);
     if (rc != NNHIP_OK) return rc;
-    if (tokens < 1) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive");
+    if (tokens < 1 || misaligned(counts)) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive and counts 4-byte aligned");
     const hipError_t e = launch_kv_advance(lane, layout, tokens, counts);
     if (e != hipSuccess) return hip_fail(e, op, lane->device, "cache advance launch");
     lane->counters.kernel_launches += 1;
@@ -878,7 +881,7 @@ int nnhip_kv_cache_read(void* handle, const nnhip_kv_cache* cache, const int32_t
     KvLayout layout;
     int rc = kv_cache_of(op, lane, cache, &layout);
     if (rc != NNHIP_OK) return rc;
-    if (tokens < 1) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive");
+    if (tokens < 1 || misaligned(first)) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive and first 4-byte aligned");
     const nnhip_rows none{nullptr, 0, 0}, k = k_out ? *k_out : none, v = v_out ? *v_out : none;
     const int64_t width = static_cast<int64_t>(layout.kv_heads) * layout.head_width;
     if (!k.data && !v.data) return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "k_out and v_out are both null");
@@ -903,8 +906,8 @@ int nnhip_cached_attention(void* handle, const nnhip_kv_cache* cache, const nnhi
     if (rc != NNHIP_OK) return rc;
     if (!d || d->struct_size != sizeof(nnhip_attention_desc))
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "descriptor is null or has the wrong struct_size");
-    if (d->tokens < 1 || d->heads < 1 || d->heads % layout.kv_heads != 0)
-        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive and heads a positive multiple of kv_heads");
+    if (d->tokens < 1 || d->heads < 1 || d->heads % layout.kv_heads != 0 || misaligned(d->counts))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "tokens must be positive, heads a positive multiple of kv_heads and counts 4-byte aligned");
     if (d->window < 0 || d->sinks < 0)
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "window and sinks must not be negative");
     if (!(d->scale >= 0.0f) || !(d->scale <= 1e30f))
@@ -937,6 +940,8 @@ int nnhip_token_log_probs(void* handle, const nnhip_log_probs_desc* d)
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "descriptor is null or has the wrong struct_size");
     if (!d->logits || d->rows < 1 || d->vocabulary < 1)
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "logits must be non-null, rows and vocabulary positive");
+    if (misaligned(d->logits) || misaligned(d->targets) || misaligned(d->log_probs) || misaligned(d->entropy) || misaligned(d->top_ids) || misaligned(d->top_log_probs))
+        return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "pointers must be 4-byte aligned");
     if (d->row_stride < d->vocabulary && !(d->rows == 1 && d->row_stride >= 0))
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "row_stride must be at least vocabulary");
     if (d->top < 0 || d->top > NNHIP_LOG_PROBS_MAX_TOP || d->top > d->vocabulary)

@@ -384,7 +384,9 @@ class QuantizedDecoder:
         return tuple(HipQuantizedMatrix.from_device(self.lane, payload.view(at, size), stacked.ggml_type, rows, stacked.input_width)
                      for at in (0, size))
 
-    def _tokens(self, tokens, least: int) -> list[int]:
+    def _tokens(self, tokens, least: int, rows: int) -> list[int]:
+        if rows < 1:
+            raise ValueError("rows must be positive.")
         ids = [int(t) for t in tokens]
         if len(ids) < least:
             raise ValueError(f"at least {least} token(s) are needed.")
@@ -396,7 +398,7 @@ class QuantizedDecoder:
     def prefill(self, tokens, rows: int = 512) -> HipBuffer:
         """Takes `tokens` into the context, `rows` at a time, and returns the logits after the last one (the buffer that
         forward_token returns)."""
-        ids = self._tokens(tokens, 1)
+        ids = self._tokens(tokens, 1, rows)
         self._room(len(ids))
         d, lane = self.descriptor, self.lane
         for at in range(0, len(ids), rows):
@@ -411,7 +413,7 @@ class QuantizedDecoder:
     def score(self, tokens, rows: int = 128) -> tuple[np.ndarray, np.ndarray]:
         """Natural log probability of every token but the first, given those before it, and the entropy of the distribution
         it was drawn from; the tokens are taken into the context."""
-        ids = self._tokens(tokens, 2)
+        ids = self._tokens(tokens, 2, rows)
         self._room(len(ids))
         d, lane = self.descriptor, self.lane
         log_probs, entropies = [], []

@@ -30,6 +30,7 @@ from .native import (KV_BLOCK_TOKENS, ROTARY_HALVES, ROTARY_PAIRS, AttentionDesc
 _STORE, _ATTENTION, _ROWS = struct.Struct("=Ii Q Qqq Qqq Qqq Qqq Q iIiI"), struct.Struct("=Ii Q Qqq Qqq iiif"), struct.Struct("=Qqq")
 assert _STORE.size == ctypes.sizeof(KvStoreDesc) and _ATTENTION.size == ctypes.sizeof(AttentionDesc)
 _NO_ROWS = (0, 0, 0)
+_LARGEST = 2**31 - 1
 
 
 class Rows:
@@ -120,8 +121,8 @@ class QuantizedKvCache:
         the device), keys turned by their positions with `rotary`.  q (heads query heads of the same tokens) is turned into
         q_out, q itself by default.  A sequence whose tokens would pass the capacity is left out."""
         cache = self._cache(layer)
-        if tokens < 1:
-            raise ValueError("tokens must be positive.")
+        if not 1 <= tokens <= _LARGEST:
+            raise ValueError("tokens must be positive and fit 32 bits.")
         kv_width = self.kv_heads * self.head_width
         counts_ptr = self._int32(counts, "counts")
         k_rows, v_rows = self._rows(k, tokens, kv_width, "k"), self._rows(v, tokens, kv_width, "v")
@@ -132,7 +133,7 @@ class QuantizedKvCache:
             turn = rotary.inv_freq._require(), rotary.width, rotary.style
         q_rows = out_rows = _NO_ROWS
         if q is not None:
-            if rotary is None or heads < 1:
+            if rotary is None or not 1 <= heads <= _LARGEST:
                 raise ValueError("q needs rotary and a positive number of heads.")
             q_rows = self._rows(q, tokens, heads * self.head_width, "q")
             out_rows = q_rows if q_out is None else self._rows(q_out, tokens, heads * self.head_width, "q_out")
@@ -150,8 +151,8 @@ class QuantizedKvCache:
         and sees the keys up to it, with window > 0 the last `window` of them and the first `sinks` tokens.  scale: 1 /
         sqrt(head_width) by default.  FP32 in and out; rows behind counts[b] are left as they are."""
         cache = self._cache(layer)
-        if tokens < 1 or heads < 1 or heads % self.kv_heads != 0:
-            raise ValueError("tokens must be positive and heads a positive multiple of kv_heads.")
+        if not 1 <= tokens <= _LARGEST or not 1 <= heads <= _LARGEST or heads % self.kv_heads != 0:
+            raise ValueError("tokens must be positive, heads a positive multiple of kv_heads, both fit 32 bits.")
         if window < 0 or sinks < 0:
             raise ValueError("window and sinks must not be negative.")
         factor = 1.0 / math.sqrt(self.head_width) if scale is None else scale
@@ -162,7 +163,7 @@ class QuantizedKvCache:
         target = out if out is not None else lane.allocate(self.sequences * tokens * width)
         try:
             _ATTENTION.pack_into(self._attention, 0, _ATTENTION.size, tokens, counts_ptr, *q_rows, *self._rows(target, tokens, width, "out"),
-                                 heads, min(window, 2**31 - 1), min(sinks, 2**31 - 1), factor)
+                                 heads, min(window, _LARGEST), min(sinks, _LARGEST), factor)
             with lane.kernel("cached_attention"):
                 check(lane._lib.nnhip_cached_attention(lane._handle, cache, self._attention), "cached_attention")
         except BaseException:
@@ -175,8 +176,8 @@ class QuantizedKvCache:
              v_out: "HipBuffer | Rows | None" = None) -> None:
         """FP32 values of tokens first[b] .. first[b] + tokens - 1 of every sequence (first: int32 on the device, 0 without)."""
         cache = self._cache(layer)
-        if tokens < 1:
-            raise ValueError("tokens must be positive.")
+        if not 1 <= tokens <= _LARGEST:
+            raise ValueError("tokens must be positive and fit 32 bits.")
         if k_out is None and v_out is None:
             raise ValueError("read needs k_out or v_out.")
         width = self.kv_heads * self.head_width

@@ -171,6 +171,15 @@ def test_limits_and_refusals(lane, tmp_path):
         assert (d.rotary_base, d.rotary_width, d.rotary_pairs, d.sliding_window, d.rotary_scaling) == (10000.0, 0, True, 0, "none")
 
 
+def test_pieces_of_no_tokens_are_refused(lane, tmp_path):
+    path, _ = _model(tmp_path, "p.gguf")
+    with _decoder(lane, path, context_length=8) as dec:
+        for call in (lambda: dec.prefill([1, 2], rows=0), lambda: dec.prefill([1, 2], rows=-1), lambda: dec.score([1, 2], rows=0)):
+            with pytest.raises(ValueError):
+                call()
+        assert dec.position == 0
+
+
 def test_metadata_of_positions(lane, tmp_path):
     from gguf_writer import write_gguf
     path, _ = _model(tmp_path, "a.gguf")

@@ -543,6 +543,32 @@ def test_refusals(lane):
         cache.reset()
 
 
+def test_refusals_of_sizes_and_alignment(lane):
+    """Counts beyond 32 bits in Python; addresses between FP32 values and positions near the largest integer in the C entry."""
+    import ctypes
+    from nntrain_amd import native
+    lib, h = lane._lib, lane._handle
+    with QuantizedKvCache(lane, 1, 2, 2, 64, 100) as cache:
+        big, counts = lane.allocate(4 * 2 * 4 * 64), lane.allocate_bytes(16)
+        off = counts.view(2, 12)
+        still = Rows(big, 0, 0)
+        for call in (lambda: cache.store(0, still, still, 2**31), lambda: cache.attention(0, still, 4, 2**31), lambda: cache.attention(0, still, 2**33),
+                     lambda: cache.read(0, 2**31, k_out=still)):
+            with pytest.raises(ValueError):
+                call()
+        freq = lane.upload_raw(Rotary.frequencies(64))
+        for call in (lambda: cache.store(0, big, big, counts=off), lambda: cache.attention(0, big, 4, counts=off), lambda: cache.advance(1, counts=off),
+                     lambda: cache.read(0, 1, first=off, k_out=big), lambda: cache.store(0, big, big, rotary=Rotary(freq.view(2, 128 - 4), 62))):
+            with pytest.raises(NnHipError):
+                call()
+        size = ctypes.c_uint64()
+        assert lib.nnhip_kv_cache_bytes(1, 1, 64, 2**30, ctypes.byref(size)) == 0 and lib.nnhip_kv_cache_bytes(1, 1, 64, 2**30 + 1, ctypes.byref(size)) != 0
+        desc = native.KvCacheDesc(ctypes.sizeof(native.KvCacheDesc), 1, 1, 64, 2**30 + 1, 0, big.ptr, counts.ptr)
+        assert lib.nnhip_kv_cache_advance(h, ctypes.byref(desc), 1, None) != 0
+        for b in (big, counts, freq):
+            b.dispose()
+
+
 def test_native_refusals(lane):
     """What the C entry refuses by itself, without reaching a launch."""
     import ctypes

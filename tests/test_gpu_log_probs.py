@@ -178,3 +178,15 @@ def test_refusals(lane):
     assert lane.counters()["kernel_launches"] == launches
     for b in (x, t):
         b.dispose()
+
+
+def test_refusal_of_addresses_between_values(lane):
+    import ctypes
+    x = lane.allocate(200)
+    good = dict(struct_size=ctypes.sizeof(LogProbsDesc), rows=2, vocabulary=50, top=1, row_stride=50, logits=x.ptr, targets=x.ptr, log_probs=x.ptr + 600,
+                entropy=x.ptr + 620, top_ids=x.ptr + 640, top_log_probs=x.ptr + 660)
+    launches = lane.counters()["kernel_launches"]
+    for name in ("logits", "targets", "log_probs", "entropy", "top_ids", "top_log_probs"):
+        assert lane._lib.nnhip_token_log_probs(lane._handle, ctypes.byref(LogProbsDesc(**{**good, name: good[name] + 2}))) != 0, name
+    assert lane.counters()["kernel_launches"] == launches
+    x.dispose()

@@ -47,3 +47,7 @@ def test_operand_checks():
             bad()
     f = Rotary.frequencies(8, 16.0)
     assert f.dtype == np.float32 and np.allclose(f, [1.0, 0.5, 0.25, 0.125])
+
+
+def test_positions_stay_away_from_the_largest_integer():
+    assert _bytes(1, 1, 64, 2**30)[0] == 0 and _bytes(1, 1, 64, 2**30 + 1)[0] == 8
