@@ -24,6 +24,7 @@ constexpr int kThreads = 256;
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 constexpr int kAlone = 8;       // new tokens that may go in without the rest of their block
+constexpr int kMoreStored = 256;        // in a mark: the block has had more tokens than the buffer holds, and its scale is theirs too
 
 struct StoreArgs {
     KvLayout cache;
@@ -220,13 +221,13 @@ __device__ __forceinline__ void store_block(const StoreArgs& a, float* tile, uin
     // (another workgroup may be reading that one; it looks for `first` alone, which this workgroup never writes over).
     const int2 mark0 = reinterpret_cast<const int2*>(marks)[0], mark1 = reinterpret_cast<const int2*>(marks)[1];
     const int buffer = mark0.x == block ? 0 : mark1.x == block ? 1 : mark0.x == first ? 1 : 0;
-    const int held_block = buffer ? mark1.x : mark0.x, held_tokens = buffer ? mark1.y : mark0.y;
+    const int held_block = buffer ? mark1.x : mark0.x, held_mark = buffer ? mark1.y : mark0.y, held_tokens = held_mark & (kMoreStored - 1);
     float* open = kv.open_values(which, pair, buffer);
     const float old_scale = from > 0 ? *scale_at : 0.0f;
     load_new<DP>(a, tile, which, b, head, block, start, from, to);
     __syncthreads();
     bool done = false;
-    if (from > 0 && to - from <= kAlone && held_block == block && held_tokens == from) {
+    if (from > 0 && to - from <= kAlone && held_block == block && held_mark == from) {
         // no new value above the block's largest: the other tokens stay as they are
         const float scale = scale_of(largest_of<DP>(tile, from, to, exchange));
         if (scale <= old_scale) {
@@ -310,7 +311,12 @@ __device__ __forceinline__ void store_block(const StoreArgs& a, float* tile, uin
         if (tid == 0) {
             marks[2 * buffer] = block;
             marks[2 * buffer + 1] = to;
+            // the other buffer's block, where this call has written over all of it
+            const int other = buffer ? mark0.x : mark1.x;
+            if (other == block || (other > first && other < block)) marks[2 * (1 - buffer) + 1] = kMoreStored;
         }
+    } else if (block == first && held_block == block && tid == 0) {
+        marks[2 * buffer + 1] = kMoreStored | min(held_tokens, from);       // the tokens behind them are this call's
     }
 }
 

@@ -72,7 +72,8 @@ struct KvLayout {
     {
         return reinterpret_cast<float*>(base + open_at) + ((static_cast<size_t>(pair) * 2 + which) * 2 + buffer) * kKvBlock * padded;
     }
-    // [2 buffers][2]: the index of the block held, the number of its tokens.  No two buffers hold the same block.
+    // [2 buffers][2]: the index of the block held, the number of its tokens (those whose values in the buffer still are the
+    // block's, plus a flag where the block went on without the buffer)
     __host__ __device__ int32_t* marks(int which, int pair) const
     {
         return reinterpret_cast<int32_t*>(base + marks_at) + (static_cast<size_t>(pair) * 2 + which) * 4;

@@ -229,6 +229,73 @@ def test_lengths_set_back_inside_and_before_the_open_block(lane):
         assert np.array_equal(got_k[0], ref.cached(b[:65])) and np.array_equal(got_v[0], ref.cached(c[:65]))
 
 
+def test_tokens_written_over_after_lengths_were_set_back_do_not_come_back(lane):
+    """A call that fills up a block and goes on leaves that block's FP32 values behind; only those before it still count."""
+    kv, width = 2, 64
+    rng = _rng(60)
+    a, b, c = (_values(rng, 200, kv, width) for _ in range(3))
+    a[32:64] *= 100
+    with QuantizedKvCache(lane, 1, 1, kv, width, 256) as cache:
+        def put(at, x):
+            cache.set_lengths([at])
+            _put(lane, cache, 0, x[None], x[None])
+            return _read(lane, cache, 0, at + len(x))[0][0]
+
+        put(0, a[:32])
+        put(32, a[32:96])                                           # into the next block
+        got = put(32, b[:1])                                        # the dropped tokens' scale goes with them
+        assert np.array_equal(got, ref.cached(np.concatenate([a[:32], b[:1]])))
+        put(10, b[:100])                                            # over the first block, whose values a buffer holds
+        full = np.concatenate([a[:10], b[:54]])
+        got = put(25, c[:1])
+        assert np.array_equal(got, ref.cached(np.concatenate([ref.cached(full)[:25], c[:1]])))
+        # a block in the middle of a call, held by a buffer from before
+        cache.reset()
+        put(0, a[:100])
+        put(100, a[100:190])                                        # the buffers hold blocks 1 and 2
+        put(3, b[:187])
+        for at in (150, 80):
+            whole = ref.cached(np.concatenate([a[:3], b[:187]])[at // 64 * 64:at // 64 * 64 + 64])
+            got = put(at, c[:1])
+            if at < 128:
+                assert np.array_equal(got[64:], ref.cached(np.concatenate([whole[:at - 64], c[:1]])))
+            else:
+                kept = np.concatenate([a[:3], b[:187]])[128:at]
+                assert np.array_equal(got[128:], ref.cached(np.concatenate([kept, c[:1]])))
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_lengths_set_back_again_and_again(lane, seed):
+    """Every token stays within what its quantisations can move it: half a step of its block each, at most one a store that
+    reached the block (and FP32 roundings, 2^-22 of the largest)."""
+    kv, width, capacity = 1, 32, 400
+    rng = _rng(61, seed)
+    truth = np.zeros((capacity, kv, width), np.float32)
+    touched, largest = np.zeros(7, int), np.zeros(7)
+    with QuantizedKvCache(lane, 1, 1, kv, width, capacity) as cache:
+        length = 0
+        for _ in range(40):
+            if rng.random() < 0.5:
+                length = max(0, length - int(rng.integers(1, 150)))
+            n = min(int(rng.choice([1, 1, 3, 8, 9, 40, 64, 100, 150])), capacity - length)
+            if n == 0:
+                continue
+            x = _values(rng, n, kv, width)
+            cache.set_lengths([length])
+            _put(lane, cache, 0, x[None], x[None])
+            truth[length:length + n] = x
+            for block in range(length // 64, (length + n - 1) // 64 + 1):
+                fresh = length <= block * 64
+                now = np.abs(x[max(0, block * 64 - length):block * 64 + 64 - length]).max()
+                touched[block], largest[block] = (1, now) if fresh else (touched[block] + 1, max(largest[block], now))
+            length += n
+            for got in _read(lane, cache, 0, length):
+                for block in range((length + 63) // 64):
+                    off = np.abs(got[0] - truth[:length])[block * 64:block * 64 + 64].max()
+                    steps = 0.5 / 127 * (1 + 1 / 127) ** touched[block]         # (a quantised value may exceed its own by half a step)
+                    assert off <= touched[block] * largest[block] * (steps + 2.0 ** -22), (seed, length, block)
+
+
 def test_read_outside_the_capacity_and_behind_the_last_token(lane):
     with QuantizedKvCache(lane, 1, 2, 1, 64, 70) as cache:
         x = _values(_rng(7), 10, 1, 64)
