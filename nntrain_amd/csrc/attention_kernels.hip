@@ -494,16 +494,19 @@ __global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_k
     }
 }
 
-// CT * 16 rows a wave, W waves; blocks staged in LDS as half precision in operand order (every fragment 1 KB in lane order: no bank is
-// asked twice), two buffers, one barrier a block; the next block's codes travel during the products.
-template <int DP, int CT, int W>
-__global__ __launch_bounds__(W * 64, 2) void attend_many_kernel(const AttendArgs a)
+// CT * 16 rows a wave, W waves a team; G teams share the rows, take every G-th block and add up at the end.  Blocks are staged in
+// LDS as half precision in operand order (every fragment 1 KB in lane order: no bank is asked twice), two buffers, one
+// barrier a block; the next block's codes travel during the products.
+template <int DP, int CT, int W, int G>
+__global__ __launch_bounds__(G * W * 64, 2) void attend_many_kernel(const AttendArgs a)
 {
     constexpr int kThreads = W * 64, kRows = CT * 16 * W, kUnits = DP * kKvBlock / 16, kPerThread = (kUnits + kThreads - 1) / kThreads;
     constexpr int kWhole = DP / 64, kFragments = DP * kKvBlock * 2 / 1024;       // KB of keys (or values) in half precision
-    extern __shared__ uint4 staged[];                                            // [2][keys, values][fragment][64]
+    extern __shared__ uint4 staged_all[];                                        // [group][2][keys, values][fragment][64]
     const KvLayout& kv = a.cache;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int team = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kThreads), tid = threadIdx.x - team * kThreads;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    uint4* staged = staged_all + team * 2 * 2 * kFragments * 64;
     // the tiles with the longest spans first, the pairs side by side
     const int pairs = kv.sequences * kv.kv_heads;
     unsigned at = blockIdx.x;
@@ -557,7 +560,7 @@ __global__ __launch_bounds__(W * 64, 2) void attend_many_kernel(const AttendArgs
         scales = scales_next;
     };
 
-    fetch(s.begin);
+    if (s.begin + team < s.end) fetch(s.begin + team);
     Rows16<DP> r[CT];
     const int row_of_wave = row0 + wave * CT * 16;
 #pragma unroll
@@ -568,13 +571,13 @@ __global__ __launch_bounds__(W * 64, 2) void attend_many_kernel(const AttendArgs
     const bool any_row = row_of_wave < s.rows;
     float running = kLeastValueScale;
     const float minus = minus_one();
-    stage(0);
+    if (s.begin + team < s.end) stage(0);
     __syncthreads();
-    for (int index = s.begin; index < s.end; ++index) {
-        const int buffer = (index - s.begin) & 1, t0 = s.block(index) * kKvBlock;
+    for (int at_block = s.begin, buffer = 0; at_block < s.end; at_block += G, buffer ^= 1) {
+        const int index = at_block + team, t0 = s.block(index) * kKvBlock;
         const float2 now = scales;
-        if (index + 1 < s.end) fetch(index + 1);
-        if (any_row && t0 <= last && (t0 + kKvBlock > low || t0 < a.sinks)) {
+        if (index + G < s.end) fetch(index + G);
+        if (index < s.end && any_row && t0 <= last && (t0 + kKvBlock > low || t0 < a.sinks)) {
             const uint4* k = staged + buffer * 2 * kFragments * 64 + lane;
             const uint4* v = k + kFragments * 64;
             floatx4 scores[CT][4];
@@ -615,25 +618,61 @@ __global__ __launch_bounds__(W * 64, 2) void attend_many_kernel(const AttendArgs
                             for (int t = 0; t < CT; ++t) r[t].o[d + u] = mma(x[u][h], part ? p_lo[t][h] : p_hi[t][h], r[t].o[d + u]);
             }
         }
-        if (index + 1 < s.end) stage(buffer ^ 1);
+        if (index + G < s.end) stage(buffer ^ 1);
         __syncthreads();
     }
     const int used = splits_used(a, s), g = lane >> 4;
+    float part[CT];                 // what the sums are scaled by
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-        const float l = column_sum(r[t].l);
+        r[t].l = column_sum(r[t].l);
+        part[t] = running * (1.0f / kPartScale);
+    }
+    if constexpr (G == 2) {
+        constexpr int kPitch = DP + 4;
+        float* sums = reinterpret_cast<float*>(staged_all);
+        float* stats = sums + kRows * kPitch;
+        const int row_in = wave * CT * 16 + (lane & 15);
+        if (team == 1) {
+#pragma unroll
+            for (int t = 0; t < CT; ++t) {
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) *reinterpret_cast<floatx4*>(&sums[(row_in + t * 16) * kPitch + d * 16 + g * 4]) = r[t].o[d] * part[t];
+                if (g == 0) {
+                    stats[2 * (row_in + t * 16)] = r[t].m;
+                    stats[2 * (row_in + t * 16) + 1] = r[t].l;
+                }
+            }
+        }
+        __syncthreads();
+        if (team == 1) return;
+#pragma unroll
+        for (int t = 0; t < CT; ++t) {
+            const float m1 = stats[2 * (row_in + t * 16)], l1 = stats[2 * (row_in + t * 16) + 1], m = fmaxf(r[t].m, m1), base = m == -INFINITY ? 0.0f : m;
+            const float mine = __builtin_amdgcn_exp2f(r[t].m - base), other = __builtin_amdgcn_exp2f(m1 - base);
+            r[t].l = r[t].l * mine + l1 * other;
+            r[t].m = m;
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d)
+                r[t].o[d] = r[t].o[d] * (part[t] * mine) + *reinterpret_cast<const floatx4*>(&sums[(row_in + t * 16) * kPitch + d * 16 + g * 4]) * other;
+            part[t] = 1.0f;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+        const float l = r[t].l;
         const int row = row_of_wave + t * 16 + (lane & 15);
         if (row >= s.rows) continue;
         if (used == 1) {
             const int i = row / a.group, h = kv_head * a.group + row % a.group;
             float* to = a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * kv.head_width;
 #pragma unroll
-            for (int d = 0; d < DP / 16; ++d) put(to, r[t].o[d] * (running * (1.0f / kPartScale)) / l, d * 16 + g * 4, kv.head_width, a.wide);
+            for (int d = 0; d < DP / 16; ++d) put(to, r[t].o[d] * part[t] / l, d * 16 + g * 4, kv.head_width, a.wide);
         } else {
             const size_t to = (static_cast<size_t>(pair) * a.tokens * a.group + row) * a.splits + split;
 #pragma unroll
             for (int d = 0; d < DP / 16; ++d)
-                *reinterpret_cast<floatx4*>(a.partial + to * DP + d * 16 + g * 4) = r[t].o[d] * (running * (1.0f / kPartScale));
+                *reinterpret_cast<floatx4*>(a.partial + to * DP + d * 16 + g * 4) = r[t].o[d] * part[t];
             if (g == 0) {
                 a.stats[2 * to] = r[t].m;
                 a.stats[2 * to + 1] = l;
@@ -706,22 +745,23 @@ __global__ __launch_bounds__(kThreads) void attend_join_kernel(const AttendArgs 
     }
 }
 
-template <int DP, int CT, int W>
+template <int DP, int CT, int W, int G>
 hipError_t launch_many(Lane* lane, const AttendArgs& a, unsigned groups)
 {
-    constexpr int kLds = 2 * 2 * DP * kKvBlock * 2;
+    constexpr int kLds = G * 2 * 2 * DP * kKvBlock * 2;
     static LdsLimit limit;
-    const hipError_t e = limit.ensure(lane->device, reinterpret_cast<const void*>(&attend_many_kernel<DP, CT, W>), kLds);
+    const hipError_t e = limit.ensure(lane->device, reinterpret_cast<const void*>(&attend_many_kernel<DP, CT, W, G>), kLds);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((attend_many_kernel<DP, CT, W>), dim3(groups), dim3(W * 64), kLds, lane->stream, a);
+    hipLaunchKernelGGL((attend_many_kernel<DP, CT, W, G>), dim3(groups), dim3(G * W * 64), kLds, lane->stream, a);
     return hipGetLastError();
 }
 
 template <int DP>
-hipError_t launch(Lane* lane, AttendArgs& a, bool few, int tiles)
+hipError_t launch(Lane* lane, const AttendArgs& a, const AttendPlan& p)
 {
+    const int tiles = p.rows_of_tile / 16;
     const unsigned groups = static_cast<unsigned>(a.cache.sequences) * static_cast<unsigned>(a.cache.kv_heads) * static_cast<unsigned>(a.row_tiles) * static_cast<unsigned>(a.splits);
-    if (few) {
+    if (p.few) {
         if constexpr (DP <= 128) {
             if (tiles == 2) {
                 hipLaunchKernelGGL((attend_few_kernel<DP, 2>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
@@ -731,8 +771,12 @@ hipError_t launch(Lane* lane, AttendArgs& a, bool few, int tiles)
         hipLaunchKernelGGL((attend_few_kernel<DP, 1>), dim3(groups), dim3(kThreads), 0, lane->stream, a);
         return hipGetLastError();
     }
-    if constexpr (DP <= 128) return tiles == 8 ? launch_many<DP, 2, 4>(lane, a, groups) : launch_many<DP, 1, 4>(lane, a, groups);
-    return launch_many<DP, 1, 8>(lane, a, groups);
+    if constexpr (DP <= 128) {
+        if (tiles == 8) return launch_many<DP, 2, 4, 1>(lane, a, groups);
+        return p.teams == 2 ? launch_many<DP, 1, 4, 2>(lane, a, groups) : launch_many<DP, 1, 4, 1>(lane, a, groups);
+    } else {
+        return launch_many<DP, 1, 8, 1>(lane, a, groups);
+    }
 }
 
 }  // namespace
@@ -748,8 +792,9 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
         p.rows_of_tile = rows <= 16 || cache.padded > 128 ? 16 : 32;
     else
         // 128 rows halve what a row costs in LDS reads and conversions, 64 fill the device twice as well: 1000 tokens of 40 heads
-        // on 8 (320 tiles of 128 rows) take 55 us with 128 and 36 with 64, 2000 tokens 103 either way, 4093 tokens 330 and 361.
-        p.rows_of_tile = cache.padded > 128 || (rows + 127) / 128 * pairs > 2 * compute_units ? 128 : 64;
+        // on 8 (320 tiles of 128 rows) take 55 us with 128 and 36 with 64, four sequences of 512 tokens behind
+        // 3000, 32 heads on 16 (512 tiles), 94 and 101, 2000 tokens of the first 101 and 103, 4093 tokens 320 and 364.
+        p.rows_of_tile = cache.padded > 128 || (rows + 127) / 128 * pairs >= 2 * compute_units ? 128 : 64;
     p.row_tiles = static_cast<int>((rows + p.rows_of_tile - 1) / p.rows_of_tile);
     // blocks a tile of rows can see at most
     int64_t blocks = cache.blocks;
@@ -762,12 +807,18 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     const int64_t groups = pairs * p.row_tiles;
     // One workgroup a compute unit: every further split costs its prologue and a partial result to add up (one token over
     // 131000, 8 pairs: 49 us with one a unit, 55 with four, 67 with eight; nothing gained for batches).  Two where blocks are
-    // small: four sequences of 30000 tokens, 16 heads of 64, take 54 us with one and 46 with two.
+    // small: four sequences of 30000 tokens, 16 heads of 64, take 54 us with one and 46 with two.  Prompts, with thousands of
+    // partial results to add up, are split only as far as whole units are free (1500 tokens behind 500, 8 heads of 128: 45 us
+    // whole, 79 in two splits and one and a half workgroups a unit; 4000 tokens of 4 heads of 64: 53 and 87).
     const int64_t wanted = static_cast<int64_t>(compute_units) * (p.few && cache.padded <= 64 ? 2 : 1);
-    int64_t splits = (wanted + groups - 1) / groups;
+    int64_t splits = p.few ? (wanted + groups - 1) / groups : wanted / groups;
     const int64_t most = blocks <= kTogether ? 1 : (blocks + p.least - 1) / p.least;
     if (splits > most) splits = most;
     p.splits = static_cast<int>(splits < 1 ? 1 : splits);
+    // Tiles that leave every compute unit at most one workgroup are taken by two teams: 2000 tokens of 8 heads on 8 take 47 us
+    // instead of 58, 1000 of 8 on 2 27 instead of 32, 64 of 32 on 8 behind 8000 41 instead of 45; with more tiles than units the
+    // two workgroups of a unit do the same (500 tokens of 40 on 8: 22 and 21).
+    p.teams = !p.few && p.rows_of_tile == 64 && groups * p.splits <= compute_units ? 2 : 1;
     if (p.splits > 1) {
         p.stats_at = static_cast<size_t>(cache.sequences) * cache.kv_heads * rows * p.splits * cache.padded;
         p.scratch_floats = p.stats_at + static_cast<size_t>(cache.sequences) * cache.kv_heads * rows * p.splits * 2;
@@ -783,15 +834,14 @@ hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhi
         return (reinterpret_cast<uintptr_t>(r.data) & 15u) == 0 && r.token_stride % 4 == 0 && r.sequence_stride % 4 == 0;
     };
     a.wide = cache.head_width % 4 == 0 && aligned(d.q) && aligned(d.out);
-    const int tiles = p.rows_of_tile / 16;
     hipError_t e;
     switch (cache.padded) {
-    case 32: e = launch<32>(lane, a, p.few, tiles); break;
-    case 64: e = launch<64>(lane, a, p.few, tiles); break;
-    case 96: e = launch<96>(lane, a, p.few, tiles); break;
-    case 128: e = launch<128>(lane, a, p.few, tiles); break;
-    case 192: e = launch<192>(lane, a, p.few, tiles); break;
-    default: e = launch<256>(lane, a, p.few, tiles); break;
+    case 32: e = launch<32>(lane, a, p); break;
+    case 64: e = launch<64>(lane, a, p); break;
+    case 96: e = launch<96>(lane, a, p); break;
+    case 128: e = launch<128>(lane, a, p); break;
+    case 192: e = launch<192>(lane, a, p); break;
+    default: e = launch<256>(lane, a, p); break;
     }
     if (e != hipSuccess || p.splits == 1) return e;
     hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>(cache.sequences) * static_cast<unsigned>(d.tokens) * static_cast<unsigned>(d.heads)),

@@ -441,6 +441,33 @@ def test_sequences_of_a_batch_do_not_influence_each_other(lane, n, heads):
             x.dispose()
 
 
+@pytest.mark.parametrize("width,window,sinks", [(32, 0, 0), (64, 30, 2), (96, 0, 0), (128, 70, 1), (192, 0, 0)])
+@pytest.mark.parametrize("sequences", [40, 65])
+def test_many_pairs_of_a_few_rows(lane, sequences, width, window, sinks):
+    """More row tiles than compute units: the forms of the prompt kernel that long prompts of many heads take."""
+    kv, heads, n, before = 8, 8, 37, 100
+    rng = _rng(62, sequences, width)
+    k, v = (rng.standard_normal((sequences, before + n, kv, width)).astype(np.float32) for _ in range(2))
+    q = rng.standard_normal((sequences, n, heads, width)).astype(np.float32)
+    counts = rng.integers(0, n + 1, sequences).astype(np.int32)
+    counts[:2] = n, 1
+    with QuantizedKvCache(lane, 1, sequences, kv, width, before + n) as cache:
+        _put(lane, cache, 0, k, v)
+        cache.set_lengths([before] * sequences)
+        qb, cb, out = lane.upload_raw(q), lane.upload_raw(counts), lane.upload_raw(np.full(q.size, 7.0, np.float32))
+        cache.attention(0, qb, heads, n, window=window, sinks=sinks, counts=cb, out=out)
+        got = lane.read(out).reshape(q.shape)
+        for b in list(range(0, sequences, 9)) + [1]:
+            c = int(counts[b])
+            kb, vb = ref.cached(k[b]), ref.cached(v[b])
+            if c:
+                want, reach = ref.attend(q[b, :c], kb, vb, before, window, sinks)
+                assert np.abs(got[b, :c] - want).max() <= _tolerance(reach, before + n, width, np.abs(vb).max()), b
+            assert np.all(got[b, c:] == 7.0)
+        for b in (qb, cb, out):
+            b.dispose()
+
+
 def test_attention_far_behind_four_gigabytes(lane):
     """One head of 256 components and 18 million tokens: the codes of its last blocks lie behind 2^32 bytes."""
     width, capacity = 256, 18 << 20
