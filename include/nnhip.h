@@ -431,7 +431,7 @@ NNHIP_API int nnhip_quant_matvec_fused(void* lane, const nnhip_fused_matvec_desc
 /* out[h, :] = v[h / (heads / kv_heads), :] for h < heads: the result of causal grouped-query attention for the first
  * token of a sequence (a single key has softmax weight 1 whatever the query), which lets a decode loop exercise every
  * projection of a layer without a key/value cache (the attention core itself, Qwen35Gpu.AttentionStep,
- * NNtrain.Core/Modules/Qwen35Gpu.Attention.cs:60-120, is outside this library).  heads must be a multiple of kv_heads.
+ * NNtrain.Core/Modules/Qwen35Gpu.Attention.cs:60-120, is nnhip_cached_attention).  heads must be a multiple of kv_heads.
  * Asynchronous. */
 NNHIP_API int nnhip_first_token_attention(void* lane, const float* v, float* out, int heads, int kv_heads, int head_width);
 
