@@ -18,8 +18,9 @@
 //
 // Two kernels.  attend_few_kernel, up to 32 rows a key/value head (decode): bound by reading the cache, so every wave walks over
 // blocks of its own, codes go from memory to registers to half precision without LDS, and the keys are split over many
-// workgroups whose partial results attend_join_kernel adds up.  attend_many_kernel (prompts): bound by the matrix cores, so
-// four waves of 32 rows share each block, converted once into LDS.
+// workgroups.  attend_many_kernel (prompts): bound by the matrix cores and the softmax beside them, so the waves of a tile share
+// each block, converted once into LDS; its keys are split where there are few tiles.  The parts are added up by
+// attend_join_few_kernel (up to eight) or attend_join_kernel.
 #include "kv_cache_layout.h"
 #include "nnhip_internal.h"
 
@@ -49,6 +50,7 @@ struct AttendArgs {
     int row_tiles;          // workgroups over the rows of a pair
     int splits;             // workgroups over the keys
     int least;              // fewest blocks a split takes
+    int together;           // so many blocks are not split
     float* partial;         // [pair][row][split][padded] sums, then [pair][row][split][2] m, l
     float* stats;
 };
@@ -64,12 +66,9 @@ struct Span {
     __device__ int block(int index) const { return index < sink_blocks ? index : index - sink_blocks + window_block; }
 };
 
-// Up to kTogether blocks are not split: a wave's four blocks take 6 us, a second launch 5.5 (one token, 32 heads on 8 of 128: over
-// 500 tokens 9 us whole and 11.4 split, over 1000 11.8 either way, over 2000 17.4 in two splits and 11.9 in eight).
-constexpr int kTogether = 16;
 __device__ __forceinline__ int blocks_of_split(const AttendArgs& a, int blocks)
 {
-    return blocks <= kTogether ? kTogether : max(a.least, (blocks + a.splits - 1) / a.splits);
+    return blocks <= a.together ? a.together : max(a.least, (blocks + a.splits - 1) / a.splits);
 }
 
 // Rows [row0, row0 + rows_of_tile) of a pair, split `split`.  The number of splits in use follows from the blocks there are.
@@ -681,6 +680,47 @@ __global__ __launch_bounds__(G * W * 64, 2) void attend_many_kernel(const Attend
     }
 }
 
+// Adds up to kFewSplits splits of rows, four components a thread, every load on its way before the first is used: what bounds
+// it is reading the partial results (8000 rows of 256 in four splits: 9.2 us; a workgroup a row takes 49).
+constexpr int kFewSplits = 8;
+__global__ __launch_bounds__(kThreads) void attend_join_few_kernel(const AttendArgs a, int rows_of_tile, int rows_of_group, unsigned all)
+{
+    const KvLayout& kv = a.cache;
+    const int quads = kv.padded / 4, row_in = static_cast<int>(threadIdx.x) / quads, d = (static_cast<int>(threadIdx.x) - row_in * quads) * 4;
+    const unsigned at = blockIdx.x * static_cast<unsigned>(rows_of_group) + row_in;
+    if (row_in >= rows_of_group || at >= all) return;
+    const unsigned rows = static_cast<unsigned>(a.tokens) * static_cast<unsigned>(a.group);
+    const int row = static_cast<int>(at % rows), pair = static_cast<int>(at / rows), b = pair / kv.kv_heads, kv_head = pair - b * kv.kv_heads;
+    const float2* stats = reinterpret_cast<const float2*>(a.stats) + static_cast<size_t>(at) * a.splits;
+    const float* partial = a.partial + static_cast<size_t>(at) * a.splits * kv.padded + d;
+    floatx4 x[kFewSplits];
+    float2 st[kFewSplits];
+#pragma unroll
+    for (int k = 0; k < kFewSplits; ++k) {
+        const int from = min(k, a.splits - 1);
+        x[k] = *reinterpret_cast<const floatx4*>(partial + from * kv.padded);
+        st[k] = stats[from];
+    }
+    const Span s = span_of(a, b, row / rows_of_tile * rows_of_tile, rows_of_tile, 0);
+    if (row >= s.rows || s.left_out) return;
+    const int used = splits_used(a, s);
+    if (used == 1) return;
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kFewSplits; ++k) m = fmaxf(m, k < used ? st[k].x : -INFINITY);
+    const float base = m == -INFINITY ? 0.0f : m;
+    floatx4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < kFewSplits; ++k)
+        if (k < used) {
+            const float weight = __builtin_amdgcn_exp2f(st[k].x - base);
+            l += st[k].y * weight;
+            sum += x[k] * weight;
+        }
+    const int i = row / a.group, h = kv_head * a.group + row % a.group;
+    put(a.out.data + b * a.out.sequence_stride + i * a.out.token_stride + h * kv.head_width, sum / l, d, kv.head_width, a.wide);
+}
+
 // Adds up the splits of one row: sum_k 2^(m_k - m) o_k / sum_k 2^(m_k - m) l_k.  32 lanes hold 128 components, eight groups of
 // them take every eighth split; the groups meet in LDS in their order.  What bounds it is a chain of memory latencies, so
 // the first 64 splits are asked for before it is known how many are in use (those that are not have no weight).
@@ -775,7 +815,7 @@ hipError_t launch(Lane* lane, const AttendArgs& a, const AttendPlan& p)
         if (tiles == 8) return launch_many<DP, 2, 4, 1>(lane, a, groups);
         return p.teams == 2 ? launch_many<DP, 1, 4, 2>(lane, a, groups) : launch_many<DP, 1, 4, 1>(lane, a, groups);
     } else {
-        return launch_many<DP, 1, 8, 1>(lane, a, groups);
+        return tiles == 8 ? launch_many<DP, 1, 8, 1>(lane, a, groups) : launch_many<DP, 1, 4, 1>(lane, a, groups);
     }
 }
 
@@ -787,38 +827,53 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     AttendPlan p{};
     const int64_t rows = static_cast<int64_t>(d.tokens) * (d.heads / cache.kv_heads);
     p.few = rows <= 32;
+    p.least = 4;
     const int64_t pairs = static_cast<int64_t>(cache.sequences) * cache.kv_heads;
-    if (p.few)
-        p.rows_of_tile = rows <= 16 || cache.padded > 128 ? 16 : 32;
-    else
+    // the most splits that a tile of rows is worth, by the blocks it can see
+    auto most_splits = [&](int rows_of_tile) {
+        int64_t blocks = cache.blocks;
+        if (d.window > 0) {
+            const int64_t seen = (static_cast<int64_t>(d.window) + rows_of_tile / (d.heads / cache.kv_heads) + 1) / kKvBlock + 2 +
+                                 (static_cast<int64_t>(d.sinks) + kKvBlock - 1) / kKvBlock;
+            blocks = blocks < seen ? blocks : seen;
+        }
+        return blocks <= p.together ? 1 : (blocks + p.least - 1) / p.least;
+    };
+    p.rows_of_tile = rows <= 16 || cache.padded > 128 ? 16 : 32;
+    // Short spans are not split: for a single token 16 blocks, which its four waves go through in about the time of a second
+    // launch (one token, 32 heads on 8 of 128: over 500 tokens 9 us whole and 11.4 split, over 1000 11.8 either way, over 2000 17.4
+    // in two splits and 11.9 in eight), 8 where blocks are larger (8 heads of 256 over 600: 17.0 and 14.3) and for prompts
+    // (8 heads on one, 1017 tokens: 26.4 with 16, 23.7 with 8; 4 on one, 390 tokens: 15.2 with 8, 16.8 with 4).
+    p.together = p.few && cache.padded * p.rows_of_tile <= 128 * 16 ? 16 : 8;
+    const int64_t tiles_of_128 = (rows + 127) / 128 * pairs;
+    if (!p.few && cache.padded <= 128) {
         // 128 rows halve what a row costs in LDS reads and conversions, 64 fill the device twice as well: 1000 tokens of 40 heads
         // on 8 (320 tiles of 128 rows) take 55 us with 128 and 36 with 64, four sequences of 512 tokens behind
         // 3000, 32 heads on 16 (512 tiles), 94 and 101, 2000 tokens of the first 101 and 103, 4093 tokens 320 and 364.
-        p.rows_of_tile = cache.padded > 128 || (rows + 127) / 128 * pairs >= 2 * compute_units ? 128 : 64;
-    p.row_tiles = static_cast<int>((rows + p.rows_of_tile - 1) / p.rows_of_tile);
-    // blocks a tile of rows can see at most
-    int64_t blocks = cache.blocks;
-    if (d.window > 0) {
-        const int64_t seen = (static_cast<int64_t>(d.window) + p.rows_of_tile / (d.heads / cache.kv_heads) + 1) / kKvBlock + 2 +
-                             (static_cast<int64_t>(d.sinks) + kKvBlock - 1) / kKvBlock;
-        blocks = blocks < seen ? blocks : seen;
+        p.rows_of_tile = tiles_of_128 >= 2 * compute_units ? 128 : 64;
+    } else if (!p.few) {
+        // A unit holds one workgroup here, of eight waves or four: 128 rows wherever they fill the units, with the splits their
+        // keys are worth (heads of 256: 4000 tokens of 16 on 4 take 229 us with 128 and 337 with 64, 1000 of 8 behind 3000 74 and
+        // 97, 819 tokens of 32 on 4 51 and 46, 1376 of 4 62 and 44, 60 of 8 on 2 behind 500 37 and 30).
+        const int64_t free = compute_units / tiles_of_128, most = most_splits(128);
+        p.rows_of_tile = tiles_of_128 * (free < 1 ? 1 : free < most ? free : most) >= compute_units ? 128 : 64;
     }
-    p.least = p.few ? kWaves : 8;
+    p.row_tiles = static_cast<int>((rows + p.rows_of_tile - 1) / p.rows_of_tile);
     const int64_t groups = pairs * p.row_tiles;
     // One workgroup a compute unit: every further split costs its prologue and a partial result to add up (one token over
     // 131000, 8 pairs: 49 us with one a unit, 55 with four, 67 with eight; nothing gained for batches).  Two where blocks are
     // small: four sequences of 30000 tokens, 16 heads of 64, take 54 us with one and 46 with two.  Prompts, with thousands of
     // partial results to add up, are split only as far as whole units are free (1500 tokens behind 500, 8 heads of 128: 45 us
-    // whole, 79 in two splits and one and a half workgroups a unit; 4000 tokens of 4 heads of 64: 53 and 87).
+    // whole, 52 in two splits and one and a half workgroups a unit; 400 tokens of 8 heads on one behind 16000: 77 and 105).
     const int64_t wanted = static_cast<int64_t>(compute_units) * (p.few && cache.padded <= 64 ? 2 : 1);
     int64_t splits = p.few ? (wanted + groups - 1) / groups : wanted / groups;
-    const int64_t most = blocks <= kTogether ? 1 : (blocks + p.least - 1) / p.least;
+    const int64_t most = most_splits(p.rows_of_tile);
     if (splits > most) splits = most;
     p.splits = static_cast<int>(splits < 1 ? 1 : splits);
     // Tiles that leave every compute unit at most one workgroup are taken by two teams: 2000 tokens of 8 heads on 8 take 47 us
     // instead of 58, 1000 of 8 on 2 27 instead of 32, 64 of 32 on 8 behind 8000 41 instead of 45; with more tiles than units the
     // two workgroups of a unit do the same (500 tokens of 40 on 8: 22 and 21).
-    p.teams = !p.few && p.rows_of_tile == 64 && groups * p.splits <= compute_units ? 2 : 1;
+    p.teams = !p.few && cache.padded <= 128 && p.rows_of_tile == 64 && groups * p.splits <= compute_units ? 2 : 1;
     if (p.splits > 1) {
         p.stats_at = static_cast<size_t>(cache.sequences) * cache.kv_heads * rows * p.splits * cache.padded;
         p.scratch_floats = p.stats_at + static_cast<size_t>(cache.sequences) * cache.kv_heads * rows * p.splits * 2;
@@ -829,7 +884,7 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
 hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhip_attention_desc& d, const AttendPlan& p, float* scratch)
 {
     AttendArgs a{cache, d.tokens, d.counts, d.q, d.out, d.heads, d.heads / cache.kv_heads, d.window, d.sinks, d.scale * 1.44269504088896340736f, false, p.row_tiles,
-                 p.splits, p.least, scratch, scratch ? scratch + p.stats_at : nullptr};
+                 p.splits, p.least, p.together, scratch, scratch ? scratch + p.stats_at : nullptr};
     auto aligned = [](const nnhip_rows& r) {
         return (reinterpret_cast<uintptr_t>(r.data) & 15u) == 0 && r.token_stride % 4 == 0 && r.sequence_stride % 4 == 0;
     };
@@ -844,8 +899,13 @@ hipError_t launch_cached_attention(Lane* lane, const KvLayout& cache, const nnhi
     default: e = launch<256>(lane, a, p); break;
     }
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL(attend_join_kernel, dim3(static_cast<unsigned>(cache.sequences) * static_cast<unsigned>(d.tokens) * static_cast<unsigned>(d.heads)),
-                       dim3(kThreads), 0, lane->stream, a, p.rows_of_tile);
+    const unsigned rows = static_cast<unsigned>(cache.sequences) * static_cast<unsigned>(d.tokens) * static_cast<unsigned>(d.heads);
+    if (p.splits <= kFewSplits) {
+        const int together = kThreads / (cache.padded / 4);
+        hipLaunchKernelGGL(attend_join_few_kernel, dim3((rows + together - 1) / together), dim3(kThreads), 0, lane->stream, a, p.rows_of_tile, together, rows);
+    } else {
+        hipLaunchKernelGGL(attend_join_kernel, dim3(rows), dim3(kThreads), 0, lane->stream, a, p.rows_of_tile);
+    }
     return hipGetLastError();
 }
 

@@ -172,7 +172,7 @@ hipError_t launch_kv_read(Lane* lane, const KvLayout& cache, const int32_t* firs
 // How an attention call is cut up (from its sizes alone, so that a captured graph keeps its form), and its scratch memory.
 struct AttendPlan {
     bool few;               // up to 32 query rows a key/value head
-    int rows_of_tile, row_tiles, splits, least, teams;
+    int rows_of_tile, row_tiles, splits, least, together, teams;
     size_t scratch_floats, stats_at;
 };
 AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_desc& d, int compute_units);

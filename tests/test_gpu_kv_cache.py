@@ -348,6 +348,16 @@ def test_attention_against_64_bits(lane, case):
     assert np.linalg.norm(got - want) <= 1e-5 * np.linalg.norm(want)
 
 
+@pytest.mark.parametrize("case", [(4, 1, 64, 3000, 1, 0, 0), (6, 2, 80, 2500, 3, 0, 0), (2, 1, 256, 2700, 1, 0, 0), (8, 1, 64, 6000, 40, 0, 0),
+                                  (3, 1, 128, 900, 50, 700, 5), (5, 1, 96, 640, 1, 0, 0), (2, 2, 192, 700, 70, 0, 0), (4, 1, 32, 2100, 33, 0, 0)],
+                         ids=lambda c: "-".join(map(str, c)))
+def test_long_spans_in_parts(lane, case):
+    """Spans of a few and of many parts, whose partial results are added up in two ways."""
+    got, want, tolerance = _attend_case(lane, *case, seed=63)
+    assert np.abs(got - want).max() <= tolerance, (np.abs(got - want).max(), tolerance)
+    assert np.linalg.norm(got - want) <= 1e-5 * np.linalg.norm(want)
+
+
 @pytest.mark.parametrize("heads,kv,n", [(4, 2, 1), (4, 1, 200)])
 def test_sharp_flat_and_zero_scales(lane, heads, kv, n):
     for scale, sharp in ((None, 12.0), (0.0, 1.0), (1e-30, 1.0), (1.0, 1e-20), (None, 1e-30), (1e-18, 1e18)):
