@@ -115,8 +115,8 @@ struct Best {
             if (v <= last) continue;
             const int32_t i = __builtin_amdgcn_readlane(index, from);
             const int place = __popcll(__ballot(value >= v));
-            const float above = __shfl_up(value, 1);
-            const int32_t above_id = __shfl_up(id, 1);
+            const float above = __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(value), 0x138, 0xf, 0xf, false));     // lane - 1
+            const int32_t above_id = __builtin_amdgcn_update_dpp(0, id, 0x138, 0xf, 0xf, false);
             value = lane < place ? value : lane == place ? v : above;
             id = lane < place ? id : lane == place ? i : above_id;
             last = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(value), top - 1));
@@ -154,7 +154,8 @@ struct Joined {
     float hand[W][kHandLogits];
     uint64_t candidates[W * NNHIP_LOG_PROBS_MAX_TOP], best[NNHIP_LOG_PROBS_MAX_TOP];
     int32_t before[kMaxPieces], chosen[NNHIP_LOG_PROBS_MAX_TOP], counts[kMaxPieces / 64], found[W];
-    float threshold;
+    float threshold, bounds[W][2];
+    int listed;
 };
 
 // The sums of the waves, in their order; every thread gets them.
@@ -178,6 +179,7 @@ __device__ void join_sums(Joined<W>& j, Sums& sums)
         sums.S += j.S[w];
         sums.T += j.T[w];
     }
+    asm volatile("" : "+v"(sums.S), "+v"(sums.T));              // added up here: 32 registers of summands would wait for the end
 }
 
 // Of the 64 keys of group `other` in LDS, those that go before key v of lane `lane` of group `group`: greater ones, and equal
@@ -187,14 +189,14 @@ __device__ __forceinline__ int places_before(const int4* keys, int other, int32_
     int before = 0;
     if (other != group) {
         const int32_t least = other < group ? v - 1 : v;
-#pragma unroll 8
+#pragma unroll 2
         for (int q = 0; q < 16; ++q) {
             const int4 x = keys[other * 16 + q];
             before += (x.x > least ? 1 : 0) + (x.y > least ? 1 : 0) + (x.z > least ? 1 : 0) + (x.w > least ? 1 : 0);
         }
         return before;
     }
-#pragma unroll 4
+#pragma unroll 2
     for (int q = 0; q < 16; ++q) {
         const int4 x = keys[other * 16 + q];
         before += (x.x > (4 * q < lane ? v - 1 : v) ? 1 : 0) + (x.y > (4 * q + 1 < lane ? v - 1 : v) ? 1 : 0) +
@@ -203,60 +205,68 @@ __device__ __forceinline__ int places_before(const int4* keys, int other, int32_
     return before;
 }
 
-// The top-th largest of the 64 lanes' values: at least `top` logits of the wave are no smaller.
-__device__ __forceinline__ float lanes_threshold(float value, int top)
+// At most the n-th largest of the 64 lanes' values and less than 2^-5 below it, for two n: the upper 14 bits of its order key,
+// one by one.
+__device__ __forceinline__ float2 nth_largest(float value, int n0, int n1)
 {
-    const int lane = threadIdx.x & 63;
-    const int32_t key = order_key(value);
-    int before = 0;
-#pragma unroll 16
-    for (int l = 0; l < 64; ++l) before += __builtin_amdgcn_readlane(key, l) > (l < lane ? key - 1 : key) ? 1 : 0;
-    return order_value(__builtin_amdgcn_readlane(key, __builtin_ctzll(__ballot(before == top - 1))));
+    const uint32_t key = static_cast<uint32_t>(order_key(value)) ^ 0x80000000u;
+    uint32_t found0 = 0, found1 = 0;
+#pragma unroll
+    for (int bit = 31; bit > 17; --bit) {
+        const uint32_t with0 = found0 | 1u << bit, with1 = found1 | 1u << bit;
+        found0 = __popcll(__ballot(key >= with0)) >= n0 ? with0 : found0;
+        found1 = __popcll(__ballot(key >= with1)) >= n1 ? with1 : found1;
+    }
+    // (keys below that of the least finite number are no numbers)
+    return float2{found0 < 0x00800000u ? -INFINITY : order_value(static_cast<int32_t>(found0 ^ 0x80000000u)),
+                  found1 < 0x00800000u ? -INFINITY : order_value(static_cast<int32_t>(found1 ^ 0x80000000u))};
 }
 
 // The `top` best logits of a row whose pieces' maxima are in LDS -> j.best, j.best_id, in their order.
 template <int W>
 __device__ void find_best(Joined<W>& j, const LogProbArgs& a, const float* x)
 {
-    constexpr int kRounds = (kMaxPieces + W * 64 - 1) / (W * 64);
+    constexpr int kRounds = (kMaxPieces + W * 64 - 1) / (W * 64), kList = W * NNHIP_LOG_PROBS_MAX_TOP;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), top = a.d.top, pieces = a.pieces;
     const int wanted = top < pieces ? top : pieces;
-    // The place of every piece among all: groups of 64 pieces against groups of 64, spread over the waves.
-    const int groups = (pieces + 63) / 64;
-    if (tid == 0) j.threshold = -INFINITY;                      // (fewer pieces than alternatives: every logit counts)
-    for (int p = tid; p < groups * 64; p += W * 64) {
-        j.before[p] = 0;
-        if (p >= pieces) j.maxima[p] = INT32_MIN;
-    }
-    __syncthreads();
-    for (int task = wave; task < groups * groups; task += W) {
-        const int group = task % groups, p = group * 64 + lane;
-        atomicAdd(&j.before[p], places_before(reinterpret_cast<const int4*>(j.maxima), task / groups, j.maxima[p], group, lane));
-    }
-    __syncthreads();
-    bool chosen[kRounds];
+    const bool choose = top < pieces;
+    if (tid == 0) j.listed = 0;
+    if (choose) {
+        // The place of every piece among all: groups of 64 pieces against groups of 64, spread over the waves.
+        const int groups = (pieces + 63) / 64;
+        for (int p = tid; p < groups * 64; p += W * 64) {
+            j.before[p] = 0;
+            if (p >= pieces) j.maxima[p] = INT32_MIN;
+        }
+        __syncthreads();
+        for (int task = wave; task < groups * groups; task += W) {
+            const int group = task % groups, p = group * 64 + lane;
+            atomicAdd(&j.before[p], places_before(reinterpret_cast<const int4*>(j.maxima), task / groups, j.maxima[p], group, lane));
+        }
+        __syncthreads();
+        bool chosen[kRounds];
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {
-        const int p = (r * W + wave) * 64 + lane;
-        chosen[r] = p < pieces && j.before[p] < wanted;
-        if (chosen[r] && j.before[p] == wanted - 1 && wanted == top) j.threshold = order_value(j.maxima[p]);
-        const uint64_t mask = __ballot(chosen[r]);
-        if (lane == 0 && r * W + wave < kMaxPieces / 64) j.counts[r * W + wave] = __popcll(mask);
-    }
-    __syncthreads();
+        for (int r = 0; r < kRounds; ++r) {
+            const int p = (r * W + wave) * 64 + lane;
+            chosen[r] = p < pieces && j.before[p] < top;
+            if (chosen[r] && j.before[p] == top - 1) j.threshold = order_value(j.maxima[p]);
+            const uint64_t mask = __ballot(chosen[r]);
+            if (lane == 0 && r * W + wave < kMaxPieces / 64) j.counts[r * W + wave] = __popcll(mask);
+        }
+        __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kRounds; ++r) {                         // in rising order
-        const uint64_t mask = __ballot(chosen[r]);
-        if (mask == 0) continue;
-        int at = __popcll(mask & ((1ull << lane) - 1));
-        for (int w = 0; w < r * W + wave; ++w) at += j.counts[w];
-        if (chosen[r]) j.chosen[at] = (r * W + wave) * 64 + lane;
+        for (int r = 0; r < kRounds; ++r) {                         // in rising order
+            const uint64_t mask = __ballot(chosen[r]);
+            if (mask == 0) continue;
+            int at = __popcll(mask & ((1ull << lane) - 1));
+            for (int w = 0; w < r * W + wave; ++w) at += j.counts[w];
+            if (chosen[r]) j.chosen[at] = (r * W + wave) * 64 + lane;
+        }
+        __syncthreads();
+    } else {
+        __syncthreads();
     }
-    __syncthreads();
-    float threshold = j.threshold;
-    Best best;
-    best.clear();
-    // piece by piece, 1024 logits at a time, the next ones on their way
+    float threshold = choose ? j.threshold : -INFINITY;
     float now[kHand], next[kHand];
     int64_t at = 0, end = 0, next_at = 0, next_end = 0;
     auto fetch = [&](float (&to)[kHand], int64_t from, int64_t until) {
@@ -266,69 +276,118 @@ __device__ void find_best(Joined<W>& j, const LogProbArgs& a, const float* x)
         for (int u = 0; u < kHand; ++u) to[u] = u * 64 + lane < left ? y[u * 64 + lane] : 0.0f;
     };
     auto open = [&](int c, int64_t& from, int64_t& until) {
-        from = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(j.chosen[c])) * a.piece;
+        from = static_cast<int64_t>(choose ? __builtin_amdgcn_readfirstlane(j.chosen[c]) : c) * a.piece;
         until = from + a.piece < a.d.vocabulary ? from + a.piece : a.d.vocabulary;
     };
     int c = wave;
-    bool c0 = true;
     if (c < wanted) {
         open(c, at, end);
         fetch(now, at, end);
     }
-    while (c < wanted) {
-        const int left = static_cast<int>(end - at < kHandLogits ? end - at : kHandLogits);
-        next_at = at + kHandLogits;
-        next_end = end;
-        if (next_at >= end) {
-            c += W;
-            if (c < wanted) open(c, next_at, next_end);
-        }
-        if (c < wanted) fetch(next, next_at, next_end);
-        if (c0 && wanted < top) {
-            // fewer pieces than alternatives: in place of the pieces' maxima those of the lanes of the wave's first piece (a row
-            // of two pieces, twenty alternatives: 23 us without, 14 with it; where there are enough pieces it costs 3 us more
-            // than it saves)
+    if (!choose) {
+        // No more pieces than alternatives: a threshold from the lanes of the waves' first pieces.  Where each of n waves has top / n
+        // lanes no smaller, the row has `top` logits no smaller; so it has where one wave has `top` of them.
+        const int waves = wanted < W ? wanted : W, each = (top + waves - 1) / waves;
+        if (wave < waves) {
+            const int left = static_cast<int>(end - at < kHandLogits ? end - at : kHandLogits);
             float most = -INFINITY;
 #pragma unroll
             for (int u = 0; u < kHand; ++u) most = u * 64 + lane < left ? (now[u] != now[u] ? INFINITY : fmaxf(most, now[u])) : most;
-            threshold = fmaxf(threshold, lanes_threshold(most, top));
-            c0 = false;
+            const float2 bounds = nth_largest(most, each, top);
+            if (lane == 0) {
+                j.bounds[wave][0] = bounds.x;
+                j.bounds[wave][1] = bounds.y;
+            }
         }
-        // which of the sixteen hold a candidate; those go through LDS, so that the code that takes one in exists once
-        uint32_t some = 0;
-#pragma unroll
-        for (int u = 0; u < kHand; ++u) {
-            some |= __any(u * 64 + lane < left && !(now[u] < threshold)) ? 1u << u : 0u;
-            j.hand[wave][u * 64 + lane] = now[u];
+        __syncthreads();
+        float least = INFINITY;
+        for (int w = 0; w < waves; ++w) {
+            least = fminf(least, j.bounds[w][0]);
+            threshold = fmaxf(threshold, j.bounds[w][1]);
         }
-        while (some) {
-            const int u = __builtin_ctz(some);
-            some &= some - 1;
-            const float v = j.hand[wave][u * 64 + lane];
-            best.offer(__ballot(u * 64 + lane < left && !(v < threshold) && !(v <= best.last)), v, static_cast<int32_t>(at) + u * 64 + lane, top);
-        }
-        at = next_at;
-        end = next_end;
-#pragma unroll
-        for (int u = 0; u < kHand; ++u) now[u] = next[u];
+        threshold = fmaxf(threshold, least);
     }
-    // the waves' entries side by side, then every entry counts those that go before it
-    const uint64_t held = __ballot(best.id >= 0);
-    if (lane == 0) j.found[wave] = __popcll(held);
-    __syncthreads();
-    int place = 0, all = 0;
-    for (int w = 0; w < W; ++w) {
-        place += w < wave ? j.found[w] : 0;
-        all += j.found[w];
+    // Piece by piece, 1024 logits at a time, the next ones on their way.  What is not below the threshold goes into one list (241
+    // rows of 13507, 32 alternatives: 22 us; sorted lists in every wave from the start 32); where that is too short (many equal
+    // logits, rows in rising order), once more with a sorted list of `top` in every wave: as many as the list has room for.
+    int all = 0;
+    for (bool listed = true;; listed = false) {
+        Best best;
+        best.clear();
+        while (c < wanted) {
+            const int left = static_cast<int>(end - at < kHandLogits ? end - at : kHandLogits);
+            next_at = at + kHandLogits;
+            next_end = end;
+            if (next_at >= end) {
+                c += W;
+                if (c < wanted) open(c, next_at, next_end);
+            }
+            if (c < wanted) fetch(next, next_at, next_end);
+            uint64_t mask[kHand];
+            int count = 0;
+#pragma unroll
+            for (int u = 0; u < kHand; ++u) {
+                mask[u] = __ballot(u * 64 + lane < left && !(now[u] < threshold));
+                count += __popcll(mask[u]);
+            }
+            if (listed && count != 0) {
+                int place = 0;
+                if (lane == 0) place = atomicAdd(&j.listed, count);         // (the order in the list has no influence)
+                place = __builtin_amdgcn_readfirstlane(place);
+#pragma unroll
+                for (int u = 0; u < kHand; ++u) {
+                    if (mask[u] == 0) continue;
+                    const int mine = place + __popcll(mask[u] & ((1ull << lane) - 1));
+                    if ((mask[u] >> lane & 1) != 0 && mine < kList)
+                        j.candidates[mine] = candidate_key(now[u] != now[u] ? INFINITY : now[u], static_cast<int32_t>(at) + u * 64 + lane);
+                    place += __popcll(mask[u]);
+                }
+            } else if (!listed) {
+                // (through LDS, so that the code that takes one in exists once)
+#pragma unroll
+                for (int u = 0; u < kHand; ++u) j.hand[wave][u * 64 + lane] = now[u];
+                for (int u = 0; u < kHand; ++u) {
+                    const float v = j.hand[wave][u * 64 + lane];
+                    best.offer(__ballot(u * 64 + lane < left && !(v < threshold) && !(v <= best.last)), v, static_cast<int32_t>(at) + u * 64 + lane, top);
+                }
+            }
+            at = next_at;
+            end = next_end;
+#pragma unroll
+            for (int u = 0; u < kHand; ++u) now[u] = next[u];
+        }
+        if (!listed) {          // the waves' entries side by side
+            const uint64_t held = __ballot(best.id >= 0);
+            if (lane == 0) j.found[wave] = __popcll(held);
+            __syncthreads();
+            int place = 0;
+            all = 0;
+            for (int w = 0; w < W; ++w) {
+                place += w < wave ? j.found[w] : 0;
+                all += j.found[w];
+            }
+            if (best.id >= 0) j.candidates[place + lane] = candidate_key(best.value, best.id);          // (entries fill the lanes from 0 on)
+            break;
+        }
+        __syncthreads();
+        all = j.listed;
+        if (all <= kList) break;
+        c = wave;
+        if (c < wanted) {
+            open(c, at, end);
+            fetch(now, at, end);
+        }
     }
-    if (best.id >= 0) j.candidates[place + lane] = candidate_key(best.value, best.id);          // (entries fill the lanes from 0 on)
     __syncthreads();
-    for (int e = tid; e < all; e += W * 64) {
-        const uint64_t key = j.candidates[e];
+    // every entry counts those that go before it, four threads a quarter each
+    for (int e = tid >> 2; e < (all + 63 & ~63); e += W * 16) {
+        const uint64_t key = e < all ? j.candidates[e] : 0;
         int before = 0;
 #pragma unroll 4
-        for (int k = 0; k < all; ++k) before += j.candidates[k] > key ? 1 : 0;
-        if (before < top) j.best[before] = key;
+        for (int k = tid & 3; k < all; k += 4) before += j.candidates[k] > key ? 1 : 0;
+        before += __shfl_xor(before, 1);
+        before += __shfl_xor(before, 2);
+        if ((tid & 3) == 0 && e < all && before < top) j.best[before] = key;
     }
     __syncthreads();
 }

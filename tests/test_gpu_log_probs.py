@@ -76,6 +76,32 @@ def test_equal_rising_and_falling_logits(lane, vocabulary):
     _check(lane, x, np.array([0, 5, 7, 3, 2, vocabulary - 1]), 64)
 
 
+@pytest.mark.parametrize("rows,vocabulary,top", [(1, 3000, 64), (300, 3000, 64), (3, 1500, 5), (2, 70000, 33), (300, 20000, 20), (1, 16384, 16)])
+def test_many_equal_logits_and_few_finite_ones(lane, rows, vocabulary, top):
+    """More logits at the threshold than any list holds, rows with fewer finite logits than alternatives, and ties between pieces."""
+    rng = np.random.default_rng([77, rows, vocabulary])
+    x = rng.integers(0, 3, (rows, vocabulary)).astype(np.float32)
+    x[0, : vocabulary // 2] = -np.inf
+    if rows > 1:
+        x[1] = -np.inf
+        x[1, rng.choice(vocabulary, top - 2, replace=False)] = rng.standard_normal(top - 2)
+        x[rows - 1] = np.sort(rng.standard_normal(vocabulary)).astype(np.float32)
+    buffer = lane.upload_raw(x)
+    got = qwen35_gpu.token_log_probs(lane, buffer, rows, vocabulary, top=top)
+    ids, lps = lane.read(got.top_ids, np.int32).reshape(rows, top), lane.read(got.top_log_probs).reshape(rows, top)
+    want, _ = ref.log_probs(x)
+    for r in range(rows):
+        order = np.argsort(-x[r], kind="stable")[:top]
+        assert np.array_equal(ids[r], order), r
+        expected = want[r, order]
+        finite = np.isfinite(expected)
+        assert np.array_equal(finite, np.isfinite(lps[r]))
+        # the logarithm of a sum of at most 2^24 exponentials, each within 2^-22 of its own, in 64 bits, and one rounding
+        assert np.abs(lps[r][finite] - expected[finite]).max() <= 2.0 ** -21 + 2.0 ** -24 * np.abs(expected[finite]).max()
+    for b in (buffer, got.entropy, got.top_ids, got.top_log_probs):
+        b.dispose()
+
+
 def test_near_certain_rows_keep_their_digits(lane):
     """The largest logit 10 .. 80 above the others: ln p of it and the entropy are tiny and relative accuracy counts."""
     vocabulary = 5000
