@@ -21,6 +21,8 @@
 // workgroups.  attend_many_kernel (prompts): bound by the matrix cores and the softmax beside them, so the waves of a tile share
 // each block, converted once into LDS; its keys are split where there are few tiles.  The parts are added up by
 // attend_join_few_kernel (up to eight) or attend_join_kernel.
+#include <algorithm>
+
 #include "kv_cache_layout.h"
 #include "nnhip_internal.h"
 
@@ -829,34 +831,38 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     p.few = rows <= 32;
     p.least = 4;
     const int64_t pairs = static_cast<int64_t>(cache.sequences) * cache.kv_heads;
-    // the most splits that a tile of rows is worth, by the blocks it can see
-    auto most_splits = [&](int rows_of_tile) {
+    // the blocks that a tile of rows can see, the most splits they are worth
+    auto blocks_of = [&](int rows_of_tile) {
         int64_t blocks = cache.blocks;
         if (d.window > 0) {
             const int64_t seen = (static_cast<int64_t>(d.window) + rows_of_tile / (d.heads / cache.kv_heads) + 1) / kKvBlock + 2 +
                                  (static_cast<int64_t>(d.sinks) + kKvBlock - 1) / kKvBlock;
             blocks = blocks < seen ? blocks : seen;
         }
-        return blocks <= p.together ? 1 : (blocks + p.least - 1) / p.least;
+        return blocks;
     };
+    auto most_splits = [&](int64_t blocks) { return blocks <= p.together ? 1 : (blocks + p.least - 1) / p.least; };
     p.rows_of_tile = rows <= 16 || cache.padded > 128 ? 16 : 32;
     // Short spans are not split: for a single token 16 blocks, which its four waves go through in about the time of a second
     // launch (one token, 32 heads on 8 of 128: over 500 tokens 9 us whole and 11.4 split, over 1000 11.8 either way, over 2000 17.4
     // in two splits and 11.9 in eight), 8 where blocks are larger (8 heads of 256 over 600: 17.0 and 14.3) and for prompts
     // (8 heads on one, 1017 tokens: 26.4 with 16, 23.7 with 8; 4 on one, 390 tokens: 15.2 with 8, 16.8 with 4).
     p.together = p.few && cache.padded * p.rows_of_tile <= 128 * 16 ? 16 : 8;
-    const int64_t tiles_of_128 = (rows + 127) / 128 * pairs;
     if (!p.few && cache.padded <= 128) {
         // 128 rows halve what a row costs in LDS reads and conversions, 64 fill the device twice as well: 1000 tokens of 40 heads
         // on 8 (320 tiles of 128 rows) take 55 us with 128 and 36 with 64, four sequences of 512 tokens behind
         // 3000, 32 heads on 16 (512 tiles), 94 and 101, 2000 tokens of the first 101 and 103, 4093 tokens 320 and 364.
-        p.rows_of_tile = tiles_of_128 >= 2 * compute_units ? 128 : 64;
+        p.rows_of_tile = (rows + 127) / 128 * pairs >= 2 * compute_units ? 128 : 64;
     } else if (!p.few) {
-        // A unit holds one workgroup here, of eight waves or four: 128 rows wherever they fill the units, with the splits their
-        // keys are worth (heads of 256: 4000 tokens of 16 on 4 take 229 us with 128 and 337 with 64, 1000 of 8 behind 3000 74 and
-        // 97, 819 tokens of 32 on 4 51 and 46, 1376 of 4 62 and 44, 60 of 8 on 2 behind 500 37 and 30).
-        const int64_t free = compute_units / tiles_of_128, most = most_splits(128);
-        p.rows_of_tile = tiles_of_128 * (free < 1 ? 1 : free < most ? free : most) >= compute_units ? 128 : 64;
+        // A unit holds one workgroup here, of eight waves or four, whose steps of a block take about 15 and 8: the form whose
+        // workgroups are through first (heads of 256, 128 and 64 rows: 4000 tokens of 16 on 4 231 and 340 us, 2357 of 4 on 2 64 and
+        // 99, 600 of 8 behind 20000 185 and 276, 1376 of 4 42 and 45, 700 of 16 on 8 48 and 37, 60 of 8 on 2 behind 500 27 and 22).
+        auto steps = [&](int rows_of_tile, int64_t step) {
+            const int64_t tiles = (rows + rows_of_tile - 1) / rows_of_tile * pairs, blocks = blocks_of(rows_of_tile);
+            const int64_t free = std::max<int64_t>(compute_units / tiles, 1), splits = std::min<int64_t>(free, most_splits(blocks));
+            return static_cast<double>(std::max<int64_t>(compute_units, tiles * splits)) * static_cast<double>((blocks + splits - 1) / splits * step);
+        };
+        p.rows_of_tile = steps(128, 15) <= steps(64, 8) ? 128 : 64;
     }
     p.row_tiles = static_cast<int>((rows + p.rows_of_tile - 1) / p.rows_of_tile);
     const int64_t groups = pairs * p.row_tiles;
@@ -867,7 +873,7 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     // whole, 52 in two splits and one and a half workgroups a unit; 400 tokens of 8 heads on one behind 16000: 77 and 105).
     const int64_t wanted = static_cast<int64_t>(compute_units) * (p.few && cache.padded <= 64 ? 2 : 1);
     int64_t splits = p.few ? (wanted + groups - 1) / groups : wanted / groups;
-    const int64_t most = most_splits(p.rows_of_tile);
+    const int64_t most = most_splits(blocks_of(p.rows_of_tile));
     if (splits > most) splits = most;
     p.splits = static_cast<int>(splits < 1 ? 1 : splits);
     // Tiles that leave every compute unit at most one workgroup are taken by two teams: 2000 tokens of 8 heads on 8 take 47 us
