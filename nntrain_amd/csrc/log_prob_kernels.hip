@@ -518,9 +518,11 @@ LogProbPlan plan_token_log_probs(const nnhip_log_probs_desc& d, int compute_unit
     const int64_t piece = (hands + kMaxPieces - 1) / kMaxPieces, pieces = (hands + piece - 1) / piece;
     p.piece = static_cast<int>(piece * kHandLogits);
     p.pieces = static_cast<int>(pieces);
-    // A few short rows are one workgroup's work each, sixteen waves in one launch: a row of 8000 takes 9.9 us instead of 12.2, 253
-    // of 6906 take 11.5 instead of 15.0; a row of 32000 would take 11.6 instead of 10.5, 2100 of 5000 81 instead of 25.
-    const bool one = pieces <= 16 && d.rows <= compute_units;
+    // A few short rows are one workgroup's work each, sixteen waves in one launch: up to 16 pieces always (250 rows of 16000, five
+    // alternatives: 11.9 us instead of 15.7), up to 32 where there is more to rank than to read (250 of 18000, five 12.6 and
+    // 16.2, twenty 19.0 and 22.5; a row of 32000 and one alternative would take 11.7 instead of 10.5, of 48000 14.5 instead of 10.4).
+    // 2100 rows of 5000 would take 81 us instead of 25.
+    const bool one = pieces <= (d.top > kWaves ? 32 : 16) && d.rows <= compute_units;
     p.waves = one && pieces > kWaves ? 16 : kWaves;
     // Otherwise eight workgroups of four waves a compute unit, none with less than a piece for each wave.
     int64_t segments = one ? 1 : 8 * static_cast<int64_t>(compute_units) / d.rows;
