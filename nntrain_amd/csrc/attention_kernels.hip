@@ -866,13 +866,17 @@ AttendPlan plan_cached_attention(const KvLayout& cache, const nnhip_attention_de
     }
     p.row_tiles = static_cast<int>((rows + p.rows_of_tile - 1) / p.rows_of_tile);
     const int64_t groups = pairs * p.row_tiles;
-    // One workgroup a compute unit: every further split costs its prologue and a partial result to add up (one token over
-    // 131000, 8 pairs: 49 us with one a unit, 55 with four, 67 with eight; nothing gained for batches).  Two where blocks are
-    // small: four sequences of 30000 tokens, 16 heads of 64, take 54 us with one and 46 with two.  Prompts, with thousands of
-    // partial results to add up, are split only as far as whole units are free (1500 tokens behind 500, 8 heads of 128: 45 us
-    // whole, 52 in two splits and one and a half workgroups a unit; 400 tokens of 8 heads on one behind 16000: 77 and 105).
-    const int64_t wanted = static_cast<int64_t>(compute_units) * (p.few && cache.padded <= 64 ? 2 : 1);
-    int64_t splits = p.few ? (wanted + groups - 1) / groups : wanted / groups;
+    // Workgroups to aim at, rounded down: one more than fit at a time and the units wait for it (17 sequences of 5 tokens behind
+    // 4768, 10 heads on 2: 39 us with 272 workgroups, 25 with 238).  One a compute unit: every further split costs its prologue and a
+    // partial result to add up (one token over 131000, 8 pairs: 48 us with one a unit, 50 with two, 54 with three), and prompts
+    // have thousands of those (1500 tokens behind 500, 8 heads of 128: 45 us whole, 52 in two splits and one and a half
+    // workgroups a unit; 400 tokens of 8 heads on one behind 16000: 77 and 105).  Two a unit for single tokens, where a unit holds two
+    // (as DP * CT in attend_few_kernel), when blocks are small (four sequences of 30000 tokens, 16 heads of 64: 54 us with one, 46
+    // with two) or one would leave a tenth of the units free (136 pairs over 8000, 5 heads each: 71 us with 136 workgroups, 64 with
+    // 272, 54 with 408; 24 pairs over 30000: 47 with 264, 37 with 240 or 504).
+    const int64_t full = groups * (compute_units / groups);
+    const bool two = p.few && cache.padded * p.rows_of_tile <= 128 * 16 && (cache.padded <= 64 || full * 10 < compute_units * 9);
+    int64_t splits = (two ? 2 : 1) * compute_units / groups;
     const int64_t most = most_splits(blocks_of(p.rows_of_tile));
     if (splits > most) splits = most;
     p.splits = static_cast<int>(splits < 1 ? 1 : splits);
