@@ -346,8 +346,18 @@ class QuantizedDecoder:
                 self._owned.append(self._prompt[name])
         return self._prompt
 
-    def _prompt_layers(self, tokens, buf: dict[str, HipBuffer]) -> None:
-        """The layers over `tokens`, all rows at once; buf["hidden"] receives the last layer's output."""
+    def _prompt_layers(self, tokens, buf: dict[str, HipBuffer], together: int) -> None:
+        """The layers over `tokens`, all rows at once; buf["hidden"] receives the last layer's output.  `together` tokens enter a
+        layer's cache at a time and attend before the next ones do."""
+        try:
+            self._all_prompt_layers(tokens, buf, together)
+        except BaseException:
+            if len(tokens) > together:
+                self.lane.fill_u32(self.cache.lengths, self.position, 1)
+            raise
+        self.position += len(tokens)
+
+    def _all_prompt_layers(self, tokens, buf: dict[str, HipBuffer], together: int) -> None:
         d, lane, n = self.descriptor, self.lane, len(tokens)
         emb, ffn, eps = d.embedding_length, d.feed_forward_length, d.rms_epsilon
         q_width, kv_width = d.head_count * d.head_width, d.kv_head_count * d.head_width
@@ -359,13 +369,21 @@ class QuantizedDecoder:
             qwen35_gpu.rms_norm(lane, hidden, L.attn_norm, n, emb, eps, out=norm)
             if L.qkv is not None:
                 L.qkv.forward(lane, norm, None, rows=n, out=qkv)
-                q, k, v = Rows(qkv, row), Rows(qkv, row, 0, q_width), Rows(qkv, row, 0, q_width + kv_width)
+                places = (0, row), (q_width, row), (q_width + kv_width, row)            # offset and stride of q, k and v
             else:
-                q, k, v = Rows(qkv, q_width), Rows(qkv, kv_width, 0, n * q_width), Rows(qkv, kv_width, 0, n * (q_width + kv_width))
-                for m, at, width in ((L.q, 0, q_width), (L.k, n * q_width, kv_width), (L.v, n * (q_width + kv_width), kv_width)):
+                places = (0, q_width), (n * q_width, kv_width), (n * (q_width + kv_width), kv_width)
+                for m, (at, width) in zip((L.q, L.k, L.v), places):
                     m.forward(lane, norm, None, rows=n, out=qkv.view(4 * at, 4 * n * width))
-            self.cache.store(i, k, v, n, rotary=self._rotary, q=q, heads=d.head_count)
-            self.cache.attention(i, q, d.head_count, n, window=self.attention_window, sinks=self.attention_sinks, out=ctx)
+            if i > 0 and n > together:
+                lane.fill_u32(self.cache.lengths, self.position, 1)                     # the layer before moved it
+            for first in range(0, n, together):
+                now = min(together, n - first)
+                q, k, v = (Rows(qkv, stride, 0, at + first * stride) for at, stride in places)
+                self.cache.store(i, k, v, now, rotary=self._rotary, q=q, heads=d.head_count)
+                self.cache.attention(i, q, d.head_count, now, window=self.attention_window, sinks=self.attention_sinks,
+                                     out=Rows(ctx, q_width, 0, first * q_width))
+                if n > together:
+                    self.cache.advance(now)
             L.o.forward(lane, ctx, None, rows=n, out=attn)
             qwen35_gpu.add_in_place(lane, hidden, attn, n * emb)
             qwen35_gpu.rms_norm(lane, hidden, L.ffn_norm, n, emb, eps, out=norm)
@@ -375,8 +393,8 @@ class QuantizedDecoder:
             qwen35_gpu.silu_multiply(lane, buf["gate"], buf["up"], n * ffn, out=buf["act"])
             L.down.forward(lane, buf["act"], None, rows=n, out=attn)
             qwen35_gpu.add_in_place(lane, hidden, attn, n * emb)
-        self.cache.advance(n)
-        self.position += n
+        if n <= together:
+            self.cache.advance(n)
 
     def _halves(self, stacked: HipQuantizedMatrix, rows: int) -> tuple[HipQuantizedMatrix, HipQuantizedMatrix]:
         """The two projections of a stack, as matrices over windows of its payload."""
@@ -397,31 +415,38 @@ class QuantizedDecoder:
 
     def prefill(self, tokens, rows: int = 512) -> HipBuffer:
         """Takes `tokens` into the context, `rows` at a time, and returns the logits after the last one (the buffer that
-        forward_token returns)."""
+        forward_token returns).  The tokens of a piece enter the 8-bit cache together, so the scale of a block covers all of
+        them when the first attends: what the context holds depends on `rows` as far as block scales do (rows=1: as
+        forward_token leaves it)."""
         ids = self._tokens(tokens, 1, rows)
         self._room(len(ids))
         d, lane = self.descriptor, self.lane
         for at in range(0, len(ids), rows):
             part = ids[at:at + rows]
             buf = self._prompt_buffers(len(part), 0)
-            self._prompt_layers(part, buf)
+            self._prompt_layers(part, buf, len(part))
         last = buf["hidden"].view(4 * (len(part) - 1) * d.embedding_length, 4 * d.embedding_length)
         qwen35_gpu.rms_norm(lane, last, self.output_norm, 1, d.embedding_length, d.rms_epsilon, out=self._norm)
         self.output.forward(lane, self._norm, None, out=self.logits)
         return self.logits
 
-    def score(self, tokens, rows: int = 128) -> tuple[np.ndarray, np.ndarray]:
+    def score(self, tokens, rows: int = 1) -> tuple[np.ndarray, np.ndarray]:
         """Natural log probability of every token but the first, given those before it, and the entropy of the distribution
-        it was drawn from; the tokens are taken into the context."""
+        it was drawn from; the tokens are taken into the context.  The projections take many tokens at a time; the cache takes
+        `rows`.  With rows=1 nothing behind a token has any influence on what precedes it.  With more, which is quicker, the
+        scale of a cache block covers the tokens of the piece behind a query too, the one whose probability is asked for among
+        them: results then depend on `rows` as far as 8-bit rounding goes, and entirely where a later token is many times larger
+        than those before it, or not finite."""
         ids = self._tokens(tokens, 2, rows)
         self._room(len(ids))
         d, lane = self.descriptor, self.lane
         log_probs, entropies = [], []
-        for at in range(0, len(ids), rows):
-            part, targets = ids[at:at + rows], ids[at + 1:at + 1 + rows]
+        batch = max(rows, 128 // rows * rows)
+        for at in range(0, len(ids), batch):
+            part, targets = ids[at:at + batch], ids[at + 1:at + 1 + batch]
             n = len(targets)
             buf = self._prompt_buffers(len(part), n)
-            self._prompt_layers(part, buf)
+            self._prompt_layers(part, buf, rows)
             if n == 0:
                 break
             qwen35_gpu.rms_norm(lane, buf["hidden"], self.output_norm, n, d.embedding_length, d.rms_epsilon, out=buf["norm"])

@@ -196,3 +196,55 @@ def test_metadata_of_positions(lane, tmp_path):
         QuantizedDecoder(lane, reader).dispose()
         with pytest.raises(NotSupportedError):
             QuantizedDecoder(lane, reader, context_length=8)
+
+
+@pytest.mark.parametrize("types", [(GGML_Q4_K,) * 3, (GGML_Q4_K, GGML_Q5_K, GGML_Q6_K)])
+def test_scores_are_those_of_token_by_token_decoding(lane, tmp_path, types):
+    """By default a token's log probability depends on the tokens before it alone: as if each had entered the context by itself."""
+    path, host = _model(tmp_path, "t.gguf", qkv_types=types)
+    tokens = list(np.random.default_rng(4).integers(0, VOCAB, 70))
+    with _decoder(lane, path) as dec:
+        log_probs, entropies = dec.score(tokens[:66])
+        cpu = CpuContext(host)
+        logits = np.concatenate([cpu.step([t]) for t in tokens[:66]])
+        want, want_entropy = ref.log_probs(logits)
+        slack = 2 * BAR * np.abs(logits).max()                          # (as above)
+        assert log_probs.shape == (65,) and dec.position == 66 and list(dec.cache.read_lengths()) == [66]
+        assert np.abs(log_probs - want[np.arange(65), tokens[1:66]]).max() <= slack
+        assert np.abs(entropies - want_entropy[:65]).max() <= slack * (1 + np.abs(want).max())
+        for t in tokens[66:]:                                           # what the context holds serves the tokens behind it
+            assert oracle.rel_l2(lane.read(dec.forward_token(int(t)), count=VOCAB), cpu.step([t])[0]) <= BAR
+
+
+def test_scores_do_not_depend_on_the_tokens_behind(lane, tmp_path):
+    path, host = _model(tmp_path, "u.gguf")
+    rng = np.random.default_rng(5)
+    tokens, other = rng.integers(0, VOCAB, 64).tolist(), rng.integers(0, VOCAB, 24).tolist()
+    with _decoder(lane, path) as dec:
+        first, _ = dec.score(tokens)
+        dec.reset()
+        second, _ = dec.score(tokens[:40] + other)
+    logits = np.concatenate([CpuContext(host).step(tokens)])
+    assert np.abs(first[:39] - second[:39]).max() <= 2 * BAR * np.abs(logits).max()
+
+
+def test_a_score_that_fails_leaves_the_context_as_it_was(lane, tmp_path, monkeypatch):
+    path, _ = _model(tmp_path, "v.gguf")
+    with _decoder(lane, path) as dec:
+        dec.prefill([1, 2, 3])
+        before = lane.read(dec.forward_token(4), count=VOCAB)
+        dec.cache.set_lengths([3])
+        dec.position = 3
+        calls, attention = [], dec.cache.attention
+
+        def failing(*args, **kw):
+            calls.append(args)
+            if len(calls) == 6:                                         # the second layer's second token
+                raise RuntimeError("stop")
+            return attention(*args, **kw)
+        monkeypatch.setattr(dec.cache, "attention", failing)
+        with pytest.raises(RuntimeError):
+            dec.score([7, 8, 9, 10])
+        monkeypatch.undo()
+        assert dec.position == 3 and list(dec.cache.read_lengths()) == [3]
+        assert np.array_equal(before, lane.read(dec.forward_token(4), count=VOCAB))
