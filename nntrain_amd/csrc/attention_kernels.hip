@@ -13,7 +13,7 @@
 //
 // Precision: the codes are integers up to 127, exact in half precision.  Queries are scaled by a power of two to at most
 // 2^14 and taken as hi + lo half-precision parts, so are the probabilities times (value scale / a running power of two above
-// the value scales) times 2^14: 22 bits below the largest, nothing lost before 2^-38 of it.  Two products for each operand pair
+// the value scales of the blocks a row has seen) times 2^14: 22 bits below the largest, nothing lost before 2^-38 of it.  Two products for each operand pair
 // instead of one is what FP32 results cost; one rounding to half precision would leave 2^-12.
 //
 // Two kernels.  attend_few_kernel, up to 32 rows a key/value head (decode): bound by reading the cache, so every wave walks over
@@ -166,6 +166,7 @@ struct Rows16 {
     floatx4 o[DP / 16];
     float c;                // what a product of the scaled query and codes is multiplied by, apart from the key scale
     float m, l;             // running maximum (in powers of two; it may lag by kSlack), this lane's part of the sum
+    float running;          // the least power of two above the value scales of the blocks the row has seen: the sums o are scaled by it
     int position, low;      // of the row; first key of its window
 
     __device__ __forceinline__ void load(const AttendArgs& a, const Span& s, int b, int kv_head, int row)
@@ -209,6 +210,7 @@ struct Rows16 {
         }
         c = most < 0x7f800000u ? a.scale * down : 0.0f;
         m = -INFINITY;
+        running = kLeastValueScale;
         l = most < 0x7f800000u ? 0.0f : __uint_as_float(0x7fc00000u);           // (a query that is not finite: its row is NaN)
         position = valid ? s.start + i : -1;        // a row that is not there sees nothing
         low = a.window > 0 && position >= a.window ? position - a.window + 1 : 0;
@@ -222,10 +224,10 @@ struct Rows16 {
 };
 
 // The softmax step of one block for CT column tiles: scores (products of scaled queries and codes) -> parts of the
-// probabilities for the second product; m, l and o of the rows move on.  `running` is the power of two that the sums o are
-// scaled by, the least one seen so far above the value scales.
+// probabilities for the second product; m, l, o and `running` of the rows move on.  A block that a row does not see leaves the
+// row's `running` alone: values of any size there cost it no digits.
 template <int DP, int CT>
-__device__ __forceinline__ void softmax_step(Rows16<DP> (&r)[CT], floatx4 (&s)[CT][4], float2 scales, int t0, bool full, int sinks, float minus, float& running,
+__device__ __forceinline__ void softmax_step(Rows16<DP> (&r)[CT], floatx4 (&s)[CT][4], float2 scales, int t0, bool full, int sinks, float minus,
                                              half8 (&p_hi)[CT][2], half8 (&p_lo)[CT][2])
 {
     const int g = (threadIdx.x & 63) >> 4;
@@ -244,13 +246,17 @@ __device__ __forceinline__ void softmax_step(Rows16<DP> (&r)[CT], floatx4 (&s)[C
                 for (int i = 0; i < 4; ++i)
                     if (!r[t].sees(t0 + 16 * j + 4 * g + i, sinks)) s[t][j][i] = -INFINITY;
     }
-    const uint32_t bits = __float_as_uint(scales.y) & 0x7f800000u;
-    const float higher = fmaxf(running, __uint_as_float(bits + 0x00800000u)), keep = running / higher, factor = scales.y * (kPartScale / higher);
-    running = higher;
-    float scale[CT], next[CT], base[CT];
-    bool moved = keep != 1.0f;
+    const float above = __uint_as_float((__float_as_uint(scales.y) & 0x7f800000u) + 0x00800000u);
+    float scale[CT], next[CT], base[CT], keep[CT], factor[CT];
+    bool moved = false;
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
+        const bool sees = full || r[t].sees_block(t0, sinks);
+        const float higher = sees ? fmaxf(r[t].running, above) : r[t].running;
+        const float inverse = __uint_as_float(0x7f000000u - __float_as_uint(higher));         // (of a power of two, exact)
+        keep[t] = r[t].running * inverse;
+        factor[t] = sees ? scales.y * (kPartScale * inverse) : 0.0f;
+        r[t].running = higher;
         // never 0: a hidden score stays at -infinity
         scale[t] = fmaxf(r[t].c * scales.x, 1e-37f);
         float top = s[t][0][0];
@@ -259,13 +265,13 @@ __device__ __forceinline__ void softmax_step(Rows16<DP> (&r)[CT], floatx4 (&s)[C
 #pragma unroll
             for (int i = 0; i < 4; ++i) top = fmaxf(top, s[t][j][i]);
         next[t] = column_max(top) * scale[t];
-        moved |= __any(next[t] > r[t].m + kSlack) != 0;
+        moved |= __any(next[t] > r[t].m + kSlack || keep[t] != 1.0f) != 0;
     }
     if (moved) {
 #pragma unroll
         for (int t = 0; t < CT; ++t) {
             next[t] = fmaxf(r[t].m, next[t]);
-            const float shrink = __builtin_amdgcn_exp2f(r[t].m - (next[t] == -INFINITY ? 0.0f : next[t])), all = shrink * keep;
+            const float shrink = __builtin_amdgcn_exp2f(r[t].m - (next[t] == -INFINITY ? 0.0f : next[t])), all = shrink * keep[t];
             r[t].l *= shrink;
             r[t].m = next[t];
 #pragma unroll
@@ -283,7 +289,7 @@ __device__ __forceinline__ void softmax_step(Rows16<DP> (&r)[CT], floatx4 (&s)[C
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const float p = __builtin_amdgcn_exp2f(fmaf(s[t][2 * h + u / 4][u % 4], scale[t], -base[t]));
-                w[u] = p * factor;
+                w[u] = p * factor[t];
                 sum += p;
             }
             split_parts(w, minus, &p_hi[t][h], &p_lo[t][h]);
@@ -395,7 +401,6 @@ __global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_k
     }
 #pragma unroll
     for (int t = 0; t < CT; ++t) r[t].load(a, s, b, kv_head, row0 + t * 16 + (lane & 15));
-    float running = kLeastValueScale;
     const float minus = minus_one();
     while (index < s.end) {
         const int t0 = s.block(index) * kKvBlock;
@@ -423,7 +428,7 @@ __global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_k
         const int next = s.block(min(index, s.end - 1));
         if (index < s.end) codes.load_keys(kv, pair, next, lane);
         half8 p_hi[CT][2], p_lo[CT][2];
-        softmax_step<DP, CT>(r, scores, scales, t0, sees_all(a, t0, s.first, s.last), a.sinks, minus, running, p_hi, p_lo);
+        softmax_step<DP, CT>(r, scores, scales, t0, sees_all(a, t0, s.first, s.last), a.sinks, minus, p_hi, p_lo);
 #pragma unroll
         for (int d = 0; d < DP / 16; d += 2) {
             half8 v[2][2];
@@ -460,7 +465,7 @@ __global__ __launch_bounds__(kThreads, DP * CT <= 128 ? 2 : 1) void attend_few_k
                 const int row = t * 16 + column;
                 float m = stats[0][row][0];
                 for (int w = 1; w < kWaves; ++w) m = fmaxf(m, stats[w][row][0]);
-                const float factor = __builtin_amdgcn_exp2f(r[t].m - (m == -INFINITY ? 0.0f : m)) * (running * (1.0f / kPartScale));
+                const float factor = __builtin_amdgcn_exp2f(r[t].m - (m == -INFINITY ? 0.0f : m)) * (r[t].running * (1.0f / kPartScale));
 #pragma unroll
                 for (int d = 0; d < DP / 16; ++d) {
                     floatx4* to = reinterpret_cast<floatx4*>(&sums[wave & 1][row * kPitch + d * 16 + g * 4]);
@@ -570,7 +575,6 @@ __global__ __launch_bounds__(G * W * 64, 2) void attend_many_kernel(const Attend
     const int first = s.start + min(row_of_wave, s.rows - 1) / a.group, last = s.start + (min(row_of_wave + CT * 16, s.rows) - 1) / a.group;
     const int low = a.window > 0 && first >= a.window ? first - a.window + 1 : 0;
     const bool any_row = row_of_wave < s.rows;
-    float running = kLeastValueScale;
     const float minus = minus_one();
     if (s.begin + team < s.end) stage(0);
     __syncthreads();
@@ -601,7 +605,7 @@ __global__ __launch_bounds__(G * W * 64, 2) void attend_many_kernel(const Attend
                     for (int j = 0; j < 4; ++j) scores[t][j] = mma(x[j], r[t].lo[step], scores[t][j]);
             }
             half8 p_hi[CT][2], p_lo[CT][2];
-            softmax_step<DP, CT>(r, scores, now, t0, sees_all(a, t0, first, last), a.sinks, minus, running, p_hi, p_lo);
+            softmax_step<DP, CT>(r, scores, now, t0, sees_all(a, t0, first, last), a.sinks, minus, p_hi, p_lo);
 #pragma unroll
             for (int d = 0; d < DP / 16; d += 2) {
                 half8 x[2][2];
@@ -627,7 +631,7 @@ __global__ __launch_bounds__(G * W * 64, 2) void attend_many_kernel(const Attend
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
         r[t].l = column_sum(r[t].l);
-        part[t] = running * (1.0f / kPartScale);
+        part[t] = r[t].running * (1.0f / kPartScale);
     }
     if constexpr (G == 2) {
         constexpr int kPitch = DP + 4;

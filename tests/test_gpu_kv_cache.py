@@ -708,3 +708,31 @@ def test_native_refusals(lane):
     assert lane.counters()["kernel_launches"] == launches
     for b in (data, lengths, rows):
         b.dispose()
+
+
+@pytest.mark.parametrize("n,heads", [(2, 1), (6, 4), (20, 2), (150, 4), (300, 1)])
+@pytest.mark.parametrize("size", [1e6, 1e12, 1e30])
+def test_large_values_of_hidden_blocks_have_no_influence(lane, n, heads, size):
+    """Rows that are worked on side by side: the first ones still see a block of very large values, or see one already that
+    begins behind the others.  Those that do not keep their accuracy."""
+    kv, width = 1, 64
+    for window, before, block in ((64, 126, 0), (64, 127, 2), (320, 382, 0), (320, 383, 6)):
+        rng = _rng(15, n, heads, block)
+        k, v, q = _values(rng, before + n, kv, width), _values(rng, before + n, kv, width), _values(rng, n, heads, width)
+        v[64 * block:64 * block + 64] *= np.float32(size)
+        with QuantizedKvCache(lane, 1, 1, kv, width, before + n) as cache:
+            _put(lane, cache, 0, k[None], v[None])
+            cache.set_lengths([before])
+            qb = lane.upload_raw(q)
+            out = cache.attention(0, qb, heads, n, window=window)
+            got = lane.read(out).reshape(n, heads, width)
+            for b in (qb, out):
+                b.dispose()
+        kq, vq = ref.cached(k), ref.cached(v)
+        want, reach = ref.attend(q, kq, vq, before, window)
+        p = before + np.arange(n)
+        sees = (p >= 64 * block) & (p - window + 1 < 64 * block + 64)
+        others = np.delete(vq, np.s_[64 * block:64 * block + 64], 0)
+        assert sees.any() and not sees.all()
+        assert np.abs(got - want)[~sees].max() <= _tolerance(reach, before + n, width, np.abs(others).max())
+        assert np.abs(got - want)[sees].max() <= _tolerance(reach, before + n, width, np.abs(vq).max())
