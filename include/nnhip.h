@@ -550,8 +550,9 @@ NNHIP_API int nnhip_cached_attention(void* lane, const nnhip_kv_cache* cache, co
  *     entropy[r]   = - sum_v p[v] ln p[v]                  (nullable)
  *     top_ids[r, 0..top), top_log_probs[r, 0..top)         the `top` (0 - NNHIP_LOG_PROBS_MAX_TOP) largest logits, largest
  *                                                          first, equal ones by index; top_log_probs is nullable.
- * rows is at most 65535.  One pass over the logits; sums are kept in 64 bits, so that the log probability of a near-certain token and the entropy of
- * a peaked row keep their FP32 accuracy.  A logit of -infinity has probability 0.  A row that holds a NaN or +infinity, or
+ * rows is at most 65535.  One pass over the logits.  The largest logit's own term, 1, is kept apart from the 64-bit sum of the
+ * others, so that the log probability of a near-certain token and the entropy of a peaked row keep their digits however small they
+ * are (an exponential below 2^-126, 87 under the largest logit, counts as 0).  A logit of -infinity has probability 0.  A row that holds a NaN or +infinity, or
  * nothing above -infinity, has NaN log probabilities and entropy; in the order of top_ids a NaN counts as +infinity.  Deterministic.
  * Scratch memory as in nnhip_cached_attention.  The reference downloads the logits and works on the host
  * (QwenGgufCommand.cs:119-157).  Asynchronous. */

@@ -1,12 +1,13 @@
 // Log probabilities of given tokens, entropy and top alternatives of rows of logits (nnhip_token_log_probs).
 //
-// With m = max x, S = sum e^(x - m), T = sum (x - m) e^(x - m):
-//     ln p[t] = (x_t - m) - ln S,    entropy = ln S - T / S.
-// S is a sum in 64 bits: the largest logit adds exactly 1 to it, so S - 1 keeps the digits that the entropy and the log
-// probability of a near-certain row consist of.  (T's terms all have one sign: 16 of them meet in FP32, those sums in 64 bits.)
+// With m = max x, R = sum e^(x - m) over all logits but one that is m, T = sum (x - m) e^(x - m):
+//     ln p[t] = (x_t - m) - ln(1 + R),    entropy = ln(1 + R) - T / (1 + R).
+// The log probability and the entropy of a near-certain row consist of R alone, so the 1 of the largest logit never enters a
+// sum: a wave leaves out one logit equal to its maximum, takes it in when a greater one comes, and so do waves and segments
+// where their sums meet.  (T's terms all have one sign: 16 of them meet in FP32, those sums in 64 bits.)
 //
 // Bound by reading the logits once.  A row is cut into segments for as many workgroups as fill the device; a wave takes
-// pieces of 1024 logits of its segment with the next piece on its way, keeps its maximum m, the sums S and T of every lane
+// pieces of 1024 logits of its segment with the next piece on its way, keeps its maximum m, the sums R and T of every lane
 // relative to it (a new maximum is rare: the sums are rescaled then), and writes down each piece's largest logit.
 //
 // The `top` best logits of a row lie in the `top` pieces with the largest maxima (equal maxima by index): any other piece has
@@ -31,7 +32,7 @@ struct LogProbArgs {
     int segments;               // of a row
     int64_t segment;            // logits of one (whole pieces)
     int pieces, piece;          // pieces of a row, logits of one (a multiple of kHandLogits)
-    double* sums;               // [row][segment][2]: S, T
+    double* sums;               // [row][segment][2]: R, T
     float* tops;                // [row][segment]: m
     int32_t* maxima;            // [row][piece], order keys
 };
@@ -124,23 +125,35 @@ struct Best {
     }
 };
 
-// The sums of some logits relative to m.
+// The sums of some logits relative to m, the largest of them (kLowest if there is none above it).  R is without one logit that is
+// m, in all the lanes together, unless m is kLowest: what one lane leaves out is not in another's.
 struct Sums {
     float m;
-    double S, T;
+    double R, T;
 
     __device__ __forceinline__ void clear()
     {
         m = kLowest;
-        S = T = 0.0;
+        R = T = 0.0;
+    }
+    // Takes in the logit that was left out.
+    __device__ __forceinline__ void whole()
+    {
+        if (m > kLowest) R += 1.0;
     }
     __device__ __forceinline__ void rescale(float next)
     {
         if (next == m) return;
+        if (m == kLowest) {                                     // nothing yet, or nothing that counts beside a greater logit
+            R *= 0.0;
+            T = R;
+            m = next;
+            return;
+        }
         const double by = static_cast<double>(m) - static_cast<double>(next), e = exp(by);
-        // (by * S first: by may be -infinity only where e is 0 and S is 0 or not a number)
-        T = e == 0.0 ? 0.0 * S : e * (T + by * S);
-        S *= e;
+        // (by * R first: by may be -infinity only where e is 0 and R is 0 or not a number)
+        T = e == 0.0 ? 0.0 * R : e * (T + by * R);
+        R *= e;
         m = next;
     }
 };
@@ -149,7 +162,7 @@ struct Sums {
 template <int W>
 struct Joined {
     float m[W];
-    double S[W], T[W];
+    double R[W], T[W];
     alignas(16) int32_t maxima[kMaxPieces];                     // order keys
     float hand[W][kHandLogits];
     uint64_t candidates[W * NNHIP_LOG_PROBS_MAX_TOP], best[NNHIP_LOG_PROBS_MAX_TOP];
@@ -167,19 +180,22 @@ __device__ void join_sums(Joined<W>& j, Sums& sums)
     __syncthreads();
     float m = j.m[0];
     for (int w = 1; w < W; ++w) m = fmaxf(m, j.m[w]);
+    if (lane == 0 && sums.m != m) sums.whole();
+    const int equal = __popcll(__ballot(lane < W && j.m[lane & (W - 1)] == m));         // waves that go on without their maximum: one of them may
     sums.rescale(m);                                            // (one exponential a wave, not W in every one)
-    const double S = wave_sum(sums.S), T = wave_sum(sums.T);
+    const double R = wave_sum(sums.R), T = wave_sum(sums.T);
     if (lane == 0) {
-        j.S[wave] = S;
+        j.R[wave] = R;
         j.T[wave] = T;
     }
     __syncthreads();
-    sums.S = sums.T = 0.0;
+    sums.R = sums.T = 0.0;
     for (int w = 0; w < W; ++w) {
-        sums.S += j.S[w];
+        sums.R += j.R[w];
         sums.T += j.T[w];
     }
-    asm volatile("" : "+v"(sums.S), "+v"(sums.T));              // added up here: 32 registers of summands would wait for the end
+    if (m > kLowest) sums.R += static_cast<double>(equal - 1);
+    asm volatile("" : "+v"(sums.R), "+v"(sums.T));              // added up here: 32 registers of summands would wait for the end
 }
 
 // Of the 64 keys of group `other` in LDS, those that go before key v of lane `lane` of group `group`: greater ones, and equal
@@ -222,7 +238,7 @@ __device__ __forceinline__ float2 nth_largest(float value, int n0, int n1)
                   found1 < 0x00800000u ? -INFINITY : order_value(static_cast<int32_t>(found1 ^ 0x80000000u))};
 }
 
-// The `top` best logits of a row whose pieces' maxima are in LDS -> j.best, j.best_id, in their order.
+// The `top` best logits of a row whose pieces' maxima are in LDS -> j.best, in their order.
 template <int W>
 __device__ void find_best(Joined<W>& j, const LogProbArgs& a, const float* x)
 {
@@ -397,8 +413,9 @@ template <int W>
 __device__ void write_row(const nnhip_log_probs_desc& d, int row, const Joined<W>& j, const Sums& sums)
 {
     const int tid = threadIdx.x;
-    const bool defined = sums.S > 0.0 && sums.S < INFINITY;     // (a NaN or +infinity among the logits makes S NaN)
-    const double log_sum = log1p(sums.S - 1.0), m = static_cast<double>(sums.m);
+    // (a NaN among the logits makes R NaN; where all are -infinity nothing is left out and R is 0)
+    const bool defined = (sums.m > kLowest || sums.R > 0.0) && sums.R < INFINITY && sums.m < INFINITY;
+    const double rest = sums.m > kLowest ? sums.R : sums.R - 1.0, log_sum = log1p(rest), m = static_cast<double>(sums.m);
     if (tid < d.top) {
         const size_t at = static_cast<size_t>(row) * d.top + tid;
         const uint64_t key = j.best[tid];
@@ -406,7 +423,7 @@ __device__ void write_row(const nnhip_log_probs_desc& d, int row, const Joined<W
         d.top_ids[at] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(key));
         if (d.top_log_probs) d.top_log_probs[at] = defined ? static_cast<float>((static_cast<double>(x) - m) - log_sum) : no_number();
     }
-    if (tid == 128 && d.entropy) d.entropy[row] = defined ? static_cast<float>(log_sum - sums.T / sums.S) : no_number();
+    if (tid == 128 && d.entropy) d.entropy[row] = defined ? static_cast<float>(log_sum - sums.T / (1.0 + rest)) : no_number();
     if (tid == 64 && d.log_probs) {
         const int32_t t = d.targets[row];
         float lp = no_number();
@@ -450,14 +467,30 @@ __global__ __launch_bounds__(W * 64) void log_probs_kernel(const LogProbArgs a)
         float most = now[0];
 #pragma unroll
         for (int u = 1; u < kHand; ++u) most = fmaxf(most, now[u]);
+        const float of_lane = most;
         most = wave_max(most);
-        if (most > sums.m) sums.rescale(most);
         float t = 0.0f;
-#pragma unroll
-        for (int u = 0; u < kHand; ++u) {
-            const float d = now[u] - sums.m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-            sums.S += static_cast<double>(e);
+        auto term = [&](float v) {
+            const float d = v - sums.m, e = __builtin_amdgcn_exp2f(d * kLog2e);
             t = fmaf(fmaxf(d, -200.0f), e, t);                  // (e is 0 long before: -infinity times 0 must not come up)
+            return e;
+        };
+        if (most > sums.m) {
+            // a new maximum: the lane that holds it leaves out its largest term
+            const int owner = __builtin_ctzll(__ballot(of_lane == most));
+            if (lane == 0) sums.whole();
+            sums.rescale(most);
+            float largest_term = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kHand; ++u) {
+                const float e = term(now[u]);
+                sums.R += static_cast<double>(fminf(largest_term, e));
+                largest_term = fmaxf(largest_term, e);
+            }
+            sums.R += static_cast<double>((t - t) + (lane == owner ? 0.0f : largest_term));         // (t - t: 0 or no number)
+        } else {
+#pragma unroll
+            for (int u = 0; u < kHand; ++u) sums.R += static_cast<double>(term(now[u]));
         }
         sums.T += static_cast<double>(t);
         if (a.d.top > 0) {
@@ -484,7 +517,7 @@ __global__ __launch_bounds__(W * 64) void log_probs_kernel(const LogProbArgs a)
         write_row(a.d, row, joined, sums);
     } else if (threadIdx.x == 0) {
         a.tops[blockIdx.x] = sums.m;
-        a.sums[2 * static_cast<size_t>(blockIdx.x)] = sums.S;
+        a.sums[2 * static_cast<size_t>(blockIdx.x)] = sums.R;
         a.sums[2 * static_cast<size_t>(blockIdx.x) + 1] = sums.T;
     }
 }
@@ -503,7 +536,11 @@ __global__ __launch_bounds__(W * 64) void log_probs_join_kernel(const LogProbArg
     sums.clear();
     // (at most 128 segments: a quarter of the pieces there can be)
     if (tid < a.segments) sums = Sums{a.tops[from + tid], a.sums[2 * (from + tid)], a.sums[2 * (from + tid) + 1]};
-    sums.rescale(wave_max(sums.m));
+    const float m = wave_max(sums.m);
+    const int equal = __popcll(__ballot(sums.m == m));          // lanes that go on without their maximum: one of them may
+    if (sums.m != m) sums.whole();
+    sums.rescale(m);
+    if ((tid & 63) == 0 && m > kLowest) sums.R += static_cast<double>(equal - 1);
     join_sums(joined, sums);
     if (a.d.top > 0) find_best(joined, a, a.d.logits + static_cast<int64_t>(blockIdx.x) * a.d.row_stride);
     write_row(a.d, blockIdx.x, joined, sums);

@@ -216,3 +216,35 @@ def test_refusal_of_addresses_between_values(lane):
         assert lane._lib.nnhip_token_log_probs(lane._handle, ctypes.byref(LogProbsDesc(**{**good, name: good[name] + 2}))) != 0, name
     assert lane.counters()["kernel_launches"] == launches
     x.dispose()
+
+
+@pytest.mark.parametrize("rows,vocabulary", [(1, 700), (3, 5000), (2, 40000), (300, 1200), (40, 262144)])
+def test_near_certain_rows_keep_their_digits_down_to_the_least_exponential(lane, rows, vocabulary):
+    """One logit 8 .. 87 above all others: ln p = -log1p(rest), rest = (V - 1) e^-gap, relative to itself however small.
+
+    A term e^-gap is off by (gap * 1.45 + 3) * 2^-24 of itself (argument, constant, exponential), the sums are 64-bit, one rounding."""
+    gaps = np.linspace(8, 87, rows).round()
+    rng = np.random.default_rng([78, rows, vocabulary])
+    at = rng.integers(0, vocabulary, rows)
+    x = np.zeros((rows, vocabulary), np.float32)
+    x[np.arange(rows), at] = gaps
+    lp, entropy, ids, top_lp = _run(lane, x, at, 1)
+    rest = (vocabulary - 1) * np.exp(-gaps)
+    bar = (gaps * 1.45 + 3) * 2.0 ** -24 + 2.0 ** -24
+    assert np.all(np.abs(lp[:, 0] / -np.log1p(rest) - 1) <= bar)
+    assert np.all(np.abs(entropy[:, 0] / (np.log1p(rest) + rest * gaps / (1 + rest)) - 1) <= 2 * bar)
+    assert np.array_equal(ids[:, 0], at) and np.array_equal(top_lp, lp)
+
+
+@pytest.mark.parametrize("vocabulary", [64, 5000, 262144])
+def test_rows_with_several_largest_logits(lane, vocabulary):
+    """Equal largest logits, in one lane, in one wave and far apart: only one of them is left out of the rest."""
+    x = np.full((4, vocabulary), -60.0, np.float32)
+    places = [[0], [0, 1], [3, vocabulary - 1], [0, 7, 20, vocabulary // 2, vocabulary - 2, vocabulary - 1]]
+    for r, p in enumerate(places):
+        x[r, p] = 1.5
+    lp, entropy, _, _ = _run(lane, x, [p[-1] for p in places], 0)
+    for r, p in enumerate(places):
+        rest = len(p) - 1 + (vocabulary - len(p)) * np.exp(-61.5)
+        want, want_entropy = -np.log1p(rest), np.log1p(rest) + (vocabulary - len(p)) * np.exp(-61.5) * 61.5 / (1 + rest)
+        assert abs(lp[r, 0] / want - 1) < 6e-6 and abs(entropy[r, 0] / want_entropy - 1) < 1.2e-5, r
