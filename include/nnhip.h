@@ -552,7 +552,9 @@ NNHIP_API int nnhip_cached_attention(void* lane, const nnhip_kv_cache* cache, co
  *                                                          first, equal ones by index; top_log_probs is nullable.
  * rows is at most 65535.  One pass over the logits.  The largest logit's own term, 1, is kept apart from the 64-bit sum of the
  * others, so that the log probability of a near-certain token and the entropy of a peaked row keep their digits however small they
- * are (an exponential below 2^-126, 87 under the largest logit, counts as 0).  A logit of -infinity has probability 0.  A row that holds a NaN or +infinity, or
+ * are.  A term is the FP32 exponential of an FP32 difference, within (|x - max x| + 4) 2^-24 of itself (below 2^-126, 87 under the
+ * largest logit, it counts as 0); the sum of (x - max x) e^(x - max x) is within 2^-20 of itself more.
+ * A logit of -infinity has probability 0.  A row that holds a NaN or +infinity, or
  * nothing above -infinity, has NaN log probabilities and entropy; in the order of top_ids a NaN counts as +infinity.  Deterministic.
  * Scratch memory as in nnhip_cached_attention.  The reference downloads the logits and works on the host
  * (QwenGgufCommand.cs:119-157).  Asynchronous. */

@@ -25,6 +25,7 @@ constexpr int kThreads = 256, kWaves = 4;
 constexpr int kHand = 16, kHandLogits = kHand * 64;         // logits a lane / a wave has in hand
 constexpr int kMaxPieces = 512;                             // pieces of a row: 1024 logits each, more in rows above 524288
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.693147180559945309417f, kLn2Low = static_cast<float>(0.693147180559945309417 - static_cast<double>(kLn2));
 constexpr float kLowest = -3.402823466e38f;
 
 struct LogProbArgs {
@@ -469,10 +470,15 @@ __global__ __launch_bounds__(W * 64) void log_probs_kernel(const LogProbArgs a)
         for (int u = 1; u < kHand; ++u) most = fmaxf(most, now[u]);
         const float of_lane = most;
         most = wave_max(most);
+        // e^d = 2^a e^(d - a ln 2) with a = fl(d log2 e): the second factor makes up for the rounding of a and of log2 e, which
+        // would cost 1.45 |d| 2^-24 of the term (512 rows of 262144: 100.8 us and 98.8 without).  The 16 products of T meet in FP32, which
+        // costs T at most 2^-20 of itself and 6e-8 in those rows (in 64 bits 101.4 us, 32 such rows 20.8 instead of 20.3).
         float t = 0.0f;
         auto term = [&](float v) {
-            const float d = v - sums.m, e = __builtin_amdgcn_exp2f(d * kLog2e);
-            t = fmaf(fmaxf(d, -200.0f), e, t);                  // (e is 0 long before: -infinity times 0 must not come up)
+            const float all = v - sums.m, d = all < -200.0f ? -200.0f : all;            // (e is 0 long before; a NaN stays one)
+            const float power = d * kLog2e, term_of_power = __builtin_amdgcn_exp2f(power);
+            const float e = fmaf(term_of_power, fmaf(-power, kLn2Low, fmaf(-power, kLn2, d)), term_of_power);
+            t = fmaf(d, e, t);
             return e;
         };
         if (most > sums.m) {

@@ -248,3 +248,23 @@ def test_rows_with_several_largest_logits(lane, vocabulary):
         rest = len(p) - 1 + (vocabulary - len(p)) * np.exp(-61.5)
         want, want_entropy = -np.log1p(rest), np.log1p(rest) + (vocabulary - len(p)) * np.exp(-61.5) * 61.5 / (1 + rest)
         assert abs(lp[r, 0] / want - 1) < 6e-6 and abs(entropy[r, 0] / want_entropy - 1) < 1.2e-5, r
+
+
+@pytest.mark.parametrize("depth", [2.7, 12.1, 20.3, 31.7, 50.9, 70.3])
+@pytest.mark.parametrize("vocabulary", [3000, 262144])
+def test_flat_tails_far_below_the_largest_logit(lane, vocabulary, depth):
+    """All logits but one the same far below it: what the exponential is off by does not average out.
+
+    x - m is exact here (m = 0).  The power of two of the hardware is within 2^-23, the factor that makes up for the argument's
+    rounding within 2^-24: 3 * 2^-24 of the rest; sixteen products with x - m meet in FP32: 16 * 2^-24 of T more; 2^-24 for the
+    result's rounding."""
+    depth = float(np.float32(depth))
+    x = np.full((1, vocabulary), -depth, np.float32)
+    x[0, 17] = 0.0
+    lp, entropy, _, top_lp = _run(lane, x, [17], 2)
+    rest = (vocabulary - 1) * np.exp(-depth)
+    total = np.log1p(rest)
+    assert abs(lp[0, 0] + total) <= 3 * 2.0 ** -24 * rest / (1 + rest) + 2.0 ** -24 * total
+    want = total + depth * rest / (1 + rest)
+    assert abs(entropy[0, 0] - want) <= 2.0 ** -24 * (3 * rest + 19 * depth * rest) / (1 + rest) + 2.0 ** -24 * want
+    assert abs(top_lp[0, 1] + depth + total) <= 3 * 2.0 ** -24 * rest / (1 + rest) + 2.0 ** -24 * (depth + total)
