@@ -186,21 +186,25 @@ __device__ __forceinline__ void load_new(const StoreArgs& a, float* tile, int wh
     }
     if (which || !a.inv_freq) return;
     __syncthreads();
-    // A thread turns one pair of up to sixteen tokens in a row: the first by its angle, each further one by one step more (a
-    // product of complex numbers in 64 bits, 2^-49 off after sixteen).
+    // A thread turns one pair of the new tokens among sixteen: every sixteenth position has its turn from its angle, each further
+    // one is a step more (a product of complex numbers in 64 bits, 2^-49 off after sixteen).  The steps are taken from that position
+    // whichever token is the call's first, so that a token's turn is the same number however the tokens arrive.
     constexpr int kRun = 16;
-    const int pairs = a.rotary_width / 2, runs = (to - from + kRun - 1) / kRun;
+    const int pairs = a.rotary_width / 2, before = from / kRun, runs = (to + kRun - 1) / kRun - before;
     for (int e = tid; e < runs * pairs; e += kThreads) {
         const int run = pairs == 1 ? e : static_cast<int>(__umulhi(static_cast<uint32_t>(e), a.pair_magic)), j = e - run * pairs;
-        int t = from + run * kRun, d0, d1;
+        int t = (before + run) * kRun, d0, d1;
         const int end = min(t + kRun, to);
         const float f = a.inv_freq[j];
         double2 r = turn_of(block * kKvBlock + t, f);
         const double2 step = t + 1 < end ? turn_of(1, f) : double2{1.0, 0.0};
         rotary_pair(a, j, &d0, &d1);
+        auto next = [&] { r = double2{fma(r.x, step.x, -r.y * step.y), fma(r.x, step.y, r.y * step.x)}; };
+#pragma unroll 1
+        for (; t < from; ++t) next();
         for (; t < end; ++t) {
             turn(&tile[t * pitch + d0], &tile[t * pitch + d1], r.x, r.y);
-            r = double2{fma(r.x, step.x, -r.y * step.y), fma(r.x, step.y, r.y * step.x)};
+            next();
         }
     }
 }

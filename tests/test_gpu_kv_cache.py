@@ -736,3 +736,25 @@ def test_large_values_of_hidden_blocks_have_no_influence(lane, n, heads, size):
         assert sees.any() and not sees.all()
         assert np.abs(got - want)[~sees].max() <= _tolerance(reach, before + n, width, np.abs(others).max())
         assert np.abs(got - want)[sees].max() <= _tolerance(reach, before + n, width, np.abs(vq).max())
+
+
+@pytest.mark.parametrize("pieces", [[13], [12, 1], [5, 8], [1] * 13, [3, 10], [13 + 3, 1]])
+def test_turned_keys_do_not_depend_on_how_the_tokens_arrive(lane, pieces):
+    """A key one of whose components lies within 2^-49 of the border between two FP32 numbers after its turn (token 6412, angle
+    6412 * 0.9): the same number whichever call brings the token, and with it the same scale of the block."""
+    width, start = 32, 6400
+    k = np.zeros((1, sum(pieces), 1, width), np.float32)
+    k[0, 12, 0, 0] = 1.2270393371582031
+    freq = lane.upload_raw(np.array([0.9], np.float32))
+    with QuantizedKvCache(lane, 1, 1, 1, width, start + k.shape[1]) as cache:
+        def stored(parts):
+            cache.set_lengths([start])
+            at = 0
+            for p in parts:
+                _put(lane, cache, 0, k[:, at:at + p], k[:, at:at + p], rotary=Rotary(freq, 2))
+                cache.advance(p)
+                at += p
+            return _read(lane, cache, 0, at, first=[start])[0][0, 12, 0]
+        got, whole = stored(pieces), stored([sum(pieces)])
+        assert np.array_equal(got, whole) and abs(got[0] / (1.2270393371582031 * np.cos(6412 * np.float64(np.float32(0.9)))) - 1) < 2.0 ** -22
+    freq.dispose()
