@@ -56,6 +56,7 @@ class DecoderDescriptor:
     rotary_pairs: bool = False      # neighbouring components turn together (architecture "llama"), else halves of the head
     sliding_window: int = 0         # 0: none
     rotary_scaling: str = "none"
+    context_refusal: str = ""       # what the file asks of attention over a context and this loop does not do; empty: nothing
 
     @staticmethod
     def inspect(reader: GgufReader) -> "DecoderDescriptor":
@@ -78,11 +79,22 @@ class DecoderDescriptor:
         token = reader.get_tensor("token_embd.weight")
         if len(token.shape) != 2:
             raise InvalidDataError("GGUF tensor 'token_embd.weight' is not a matrix.")
+        refusals: list[str] = []            # (a loop without a context runs whatever these say)
+
+        def number(key: str, default, kind=int):
+            value = md.get(f"{arch}.{key}")
+            if value is None:
+                return default
+            if isinstance(value, (str, list)) or not 0 <= value < (2**31 if kind is int else float("inf")):
+                refusals.append(f"GGUF metadata '{arch}.{key}' is not one finite number from 0 on.")
+                return default
+            return kind(value)
+
         d = DecoderDescriptor(arch, need("block_count"), emb, need("feed_forward_length"), heads, kv, head_width,
                               need("attention.layer_norm_rms_epsilon", float), int(token.shape[1]),
-                              float(md.get(f"{arch}.rope.freq_base", 10000.0)), int(md.get(f"{arch}.rope.dimension_count", 0)),
-                              arch == "llama", int(md.get(f"{arch}.attention.sliding_window", 0)),
-                              str(md.get(f"{arch}.rope.scaling.type", "none")))
+                              number("rope.freq_base", 10000.0, float), number("rope.dimension_count", 0),
+                              arch == "llama", number("attention.sliding_window", 0),
+                              str(md.get(f"{arch}.rope.scaling.type", "none")), " ".join(refusals))
         if min(d.layer_count, d.embedding_length, d.feed_forward_length, d.head_count, d.kv_head_count, d.head_width) <= 0:
             raise InvalidDataError("GGUF decoder dimensions must be positive.")
         if d.head_count % d.kv_head_count != 0:
@@ -140,6 +152,8 @@ class QuantizedDecoder:
             raise ValueError("context_length, attention_window and attention_sinks must not be negative.")
         if self.context_length > 0 and descriptor.rotary_scaling != "none":
             raise NotSupportedError(f"Rotary scaling '{descriptor.rotary_scaling}' is not supported.")
+        if self.context_length > 0 and descriptor.context_refusal:
+            raise NotSupportedError(descriptor.context_refusal)
         self.cache: QuantizedKvCache | None = None
         self.position = 0           # tokens of the context so far
         self.lane = lane
@@ -213,7 +227,7 @@ class QuantizedDecoder:
             try:
                 self.cache = own(QuantizedKvCache(lane, d.layer_count, 1, d.kv_head_count, d.head_width, self.context_length))
                 width = d.rotary_width or d.head_width
-                if width > d.head_width or width % 2 != 0 or not d.rotary_base > 0:
+                if not 2 <= width <= d.head_width or width % 2 != 0 or not d.rotary_base > 0:
                     raise InvalidDataError("rope.dimension_count must be even and within a head, rope.freq_base positive.")
                 self._rotary = Rotary(own(lane.upload_raw(Rotary.frequencies(width, d.rotary_base))), width, d.rotary_pairs)
                 self._next = own(lane.allocate_bytes(4)), own(lane.allocate(1)), own(lane.allocate(1))
