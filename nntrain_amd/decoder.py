@@ -37,6 +37,15 @@ from .native import POST_SILU_PAIR
 from .quantized_matrix import PRE_RMS_NORM, PRE_SILU_MULTIPLY, HipQuantizedMatrix
 
 
+# Which components of a head turn together: neighbours (True) or those half the rotary width apart (False).  Files of other
+# architectures may hold the same tensors and pair them either way, so none is assumed for them.
+_NEIGHBOURS_TURN = {"llama": True, "qwen2": False}
+
+# Metadata of attention that this loop does not carry out, and the value at which it asks for nothing.
+_NEUTRAL = {"rope.scale_linear": 1, "attention.scale": None, "attn_logit_softcapping": 0, "attention.max_alibi_bias": 0, "attention.clamp_kqv": 0,
+            "attention.causal": True, "attention.sliding_window_pattern": None}
+
+
 @dataclass(frozen=True)
 class DecoderDescriptor:
     """The metadata a llama-style GGUF file gives for this loop (Qwen35Gguf.Inspect keeps the same fields,
@@ -53,7 +62,7 @@ class DecoderDescriptor:
     # what attention over a context needs besides (llama.cpp's keys and their defaults)
     rotary_base: float = 10000.0
     rotary_width: int = 0           # 0: head_width
-    rotary_pairs: bool = False      # neighbouring components turn together (architecture "llama"), else halves of the head
+    rotary_pairs: bool = False      # neighbouring components turn together, else halves of the head
     sliding_window: int = 0         # 0: none
     rotary_scaling: str = "none"
     context_refusal: str = ""       # what the file asks of attention over a context and this loop does not do; empty: nothing
@@ -80,6 +89,14 @@ class DecoderDescriptor:
         if len(token.shape) != 2:
             raise InvalidDataError("GGUF tensor 'token_embd.weight' is not a matrix.")
         refusals: list[str] = []            # (a loop without a context runs whatever these say)
+        if arch not in _NEIGHBOURS_TURN:
+            refusals.append(f"Rotary positions of architecture '{arch}' are not known.")
+        refusals += [f"GGUF metadata '{arch}.{key}' is not supported with a context." for key, neutral in _NEUTRAL.items()
+                     if md.get(f"{arch}.{key}", neutral) != neutral]
+        if f"{arch}.rope.scaling.type" not in md and md.get(f"{arch}.rope.scaling.factor", 1) != 1:
+            refusals.append("Rotary scaling is not supported.")             # (a factor alone scales positions)
+        if arch != "llama" and md.get(f"{arch}.attention.sliding_window", 0) != 0:
+            refusals.append(f"Which layers of architecture '{arch}' have a sliding window is not known.")
 
         def number(key: str, default, kind=int):
             value = md.get(f"{arch}.{key}")
@@ -93,7 +110,7 @@ class DecoderDescriptor:
         d = DecoderDescriptor(arch, need("block_count"), emb, need("feed_forward_length"), heads, kv, head_width,
                               need("attention.layer_norm_rms_epsilon", float), int(token.shape[1]),
                               number("rope.freq_base", 10000.0, float), number("rope.dimension_count", 0),
-                              arch == "llama", number("attention.sliding_window", 0),
+                              _NEIGHBOURS_TURN.get(arch, False), number("attention.sliding_window", 0),
                               str(md.get(f"{arch}.rope.scaling.type", "none")), " ".join(refusals))
         if min(d.layer_count, d.embedding_length, d.feed_forward_length, d.head_count, d.kv_head_count, d.head_width) <= 0:
             raise InvalidDataError("GGUF decoder dimensions must be positive.")

@@ -248,3 +248,20 @@ def test_a_score_that_fails_leaves_the_context_as_it_was(lane, tmp_path, monkeyp
         monkeypatch.undo()
         assert dec.position == 3 and list(dec.cache.read_lengths()) == [3]
         assert np.array_equal(before, lane.read(dec.forward_token(4), count=VOCAB))
+
+
+def test_an_architecture_that_turns_halves_of_a_head(lane, tmp_path, monkeypatch):
+    from gguf_writer import write_gguf
+    path, host = _model(tmp_path, "h.gguf")
+    with GgufReader(path) as reader:
+        kvs = [_kv(k.replace("llama.", "qwen2."), "qwen2" if k == "general.architecture" else v) for k, v in reader.metadata.items()
+               if k.startswith("llama") or k == "general.architecture"]
+        tensors = [(t.name, t.shape, t.type, bytes(reader.read_tensor_bytes(t))) for t in reader.tensors]
+    path = write_gguf(tmp_path / "i.gguf", tensors, kvs)
+    rotate = ref.rotate
+    monkeypatch.setattr(ref, "rotate", lambda x, at, inv, width, pairs: rotate(x, at, inv, width, pairs=False))
+    tokens = [int(t) for t in np.random.default_rng(6).integers(0, VOCAB, 12)]
+    with _decoder(lane, path) as dec:
+        cpu = CpuContext(host)
+        for t in tokens:
+            assert oracle.rel_l2(lane.read(dec.forward_token(t), count=VOCAB), cpu.step([t])[0]) <= BAR

@@ -55,3 +55,30 @@ def test_metadata_of_a_plain_file(tmp_path):
     d = _inspect(tmp_path, rope__freq_base=5e5, rope__dimension_count=16, attention__sliding_window=7)
     assert (d.rotary_base, d.rotary_width, d.sliding_window, d.context_refusal) == (5e5, 16, 7, "")
     assert not _refuses(d) and not _refuses(d, context_length=8)
+
+
+@pytest.mark.parametrize("arch,pairs", [("llama", True), ("qwen2", False)])
+def test_pairing_follows_a_table_of_architectures(tmp_path, arch, pairs):
+    d = _inspect(tmp_path, arch)
+    assert d.rotary_pairs == pairs and not _refuses(d, context_length=8)
+
+
+@pytest.mark.parametrize("arch,more", [("another", {}), ("qwen2", {"attention__sliding_window": 512}), ("llama", {"rope__scale_linear": 4.0}),
+                                       ("llama", {"rope__scaling__factor": 4.0}), ("llama", {"attention__sliding_window_pattern": [True, False]}),
+                                       ("llama", {"attention__sliding_window_pattern": 6}), ("llama", {"attn_logit_softcapping": 50.0}),
+                                       ("llama", {"attention__causal": False}), ("llama", {"attention__scale": 0.25})])
+def test_attention_that_the_loop_does_not_carry_out_is_refused_with_a_context(tmp_path, arch, more):
+    d = _inspect(tmp_path, arch, **more)
+    assert not _refuses(d) and _refuses(d, context_length=8)
+
+
+def test_metadata_that_asks_for_nothing_is_no_reason_to_refuse(tmp_path):
+    d = _inspect(tmp_path, rope__scale_linear=1.0, rope__scaling__factor=1.0, attention__causal=True, attn_logit_softcapping=0.0)
+    assert not d.context_refusal and not _refuses(d, context_length=8)
+    d = _inspect(tmp_path, rope__scaling__type="none", rope__scaling__factor=8.0)
+    assert not _refuses(d, context_length=8)
+
+
+def test_a_descriptor_that_states_its_pairing_is_taken_at_its_word():
+    d = DecoderDescriptor("another", 1, 64, 64, 2, 1, 32, 1e-5, 32, rotary_pairs=True)
+    assert not _refuses(d, context_length=8)
