@@ -97,10 +97,10 @@ class QuantizedKvCache:
     def set_lengths(self, lengths) -> None:
         """The tokens each sequence holds; smaller than before drops the last ones."""
         self._cache(0)
-        values = np.ascontiguousarray(lengths, dtype=np.int32)
-        if values.shape != (self.sequences,) or values.min() < 0 or values.max() > self.capacity:
-            raise ValueError("lengths must be one value of 0 .. capacity for each sequence.")
-        self.lane.write(self.lengths, values)
+        values = np.asarray(lengths)            # (checked before they are made 32 bits wide)
+        if values.dtype.kind not in "biuf" or values.shape != (self.sequences,) or not np.all((values >= 0) & (values <= self.capacity) & (values % 1 == 0)):
+            raise ValueError("lengths must be one whole number of 0 .. capacity for each sequence.")
+        self.lane.write(self.lengths, values.astype(np.int32))
 
     def read_lengths(self) -> np.ndarray:
         self._cache(0)

@@ -51,3 +51,22 @@ def test_operand_checks():
 
 def test_positions_stay_away_from_the_largest_integer():
     assert _bytes(1, 1, 64, 2**30)[0] == 0 and _bytes(1, 1, 64, 2**30 + 1)[0] == 8
+
+
+def test_lengths_are_checked_before_they_are_narrowed():
+    from nntrain_amd import QuantizedKvCache
+
+    class Lane:
+        disposed = False
+
+        def write(self, buffer, values):
+            self.written = values
+    cache = QuantizedKvCache.__new__(QuantizedKvCache)
+    cache.lane, cache.layers, cache.sequences, cache.capacity, cache.lengths = Lane(), 1, 2, 100, None
+    cache._owned, cache._refs = [None], [None]
+    for bad in ([0, 2**32], np.array([2**32 + 5, 1]), np.array([2**64 - 1, 0], np.uint64), [1.5, 2.0], [np.nan, 0.0], [0, -1], [0, 101], [[0, 1]], [1], ["0", "1"]):
+        with pytest.raises(ValueError):
+            cache.set_lengths(bad)
+    for good in ([0, 100], (3, 4), np.array([7, 100], np.int64), np.array([1, 2], np.uint8), np.zeros(2)):
+        cache.set_lengths(good)
+        assert cache.lane.written.dtype == np.int32 and list(cache.lane.written) == list(good)
