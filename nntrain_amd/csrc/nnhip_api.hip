@@ -767,6 +767,9 @@ static int lane_scratch(uint32_t op, nnhip::Lane* lane, size_t bytes, void** out
 
 // --- 8-bit key/value cache ---------------------------------------------------------------------------------------
 
+// A launch holds fewer than 2^32 threads: workgroups of at most 512 (attention), of 256 (the cache's own kernels).
+constexpr int64_t kMostAttentionGroups = (1ll << 32) / 512 - 1, kMostCacheGroups = (1ll << 32) / 256 - 1;
+
 static bool misaligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) != 0; }
 
 // Checks a cache descriptor and derives its layout.
@@ -851,7 +854,8 @@ int nnhip_kv_cache_store(void* handle, const nnhip_kv_cache* cache, const nnhip_
         return fail(NNHIP_ERR_INVALID_ARGUMENT, op, lane->device, 0, "heads and q_out need q");
     }
     const int64_t pairs = static_cast<int64_t>(layout.sequences) * layout.kv_heads;
-    if (pairs * 2 * (d->tokens / kKvBlock + 2) + static_cast<int64_t>(layout.sequences) * d->tokens > 0x7fffffff || kv_width > 0x3fffffff)
+    const int64_t query_groups = d->q.data ? static_cast<int64_t>(layout.sequences) * d->tokens : 0;
+    if (pairs * 2 * (d->tokens / kKvBlock + 2) + query_groups > kMostCacheGroups || kv_width > 0x3fffffff)
         return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, heads and tokens exceed one launch");
     const hipError_t e = launch_kv_store(lane, layout, *d);
     if (e != hipSuccess) return hip_fail(e, op, lane->device, "cache store launch");
@@ -889,7 +893,7 @@ int nnhip_kv_cache_read(void* handle, const nnhip_kv_cache* cache, const int32_t
     if (rc == NNHIP_OK && v.data) rc = check_rows(op, lane, v, layout.sequences, tokens, width, true, "v_out");
     if (rc != NNHIP_OK) return rc;
     const int64_t pairs = static_cast<int64_t>(layout.sequences) * layout.kv_heads;
-    if (pairs * 2 * (tokens / kKvBlock + 2) > 0x7fffffff || static_cast<int64_t>(layout.sequences) * tokens > 0x7fffffff || width > 0x3fffffff)
+    if (pairs * 2 * (tokens / kKvBlock + 2) > kMostCacheGroups || width > 0x3fffffff)
         return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, heads and tokens exceed one launch");
     const hipError_t e = launch_kv_read(lane, layout, first, tokens, k, v);
     if (e != hipSuccess) return hip_fail(e, op, lane->device, "cache read launch");
@@ -921,6 +925,8 @@ int nnhip_cached_attention(void* handle, const nnhip_kv_cache* cache, const nnhi
         return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, tokens and heads exceed one launch");
     // partial results of the splits live in the lane's scratch memory between the two launches
     const AttendPlan plan = plan_cached_attention(layout, *d, lane->compute_units);
+    if (static_cast<int64_t>(layout.sequences) * layout.kv_heads * plan.row_tiles > kMostAttentionGroups / plan.splits)
+        return fail(NNHIP_ERR_TOO_LARGE, op, lane->device, 0, "sequences, tokens and heads exceed one launch");
     void* scratch = nullptr;
     if (plan.scratch_floats) {
         rc = lane_scratch(op, lane, plan.scratch_floats * sizeof(float), &scratch);

@@ -758,3 +758,25 @@ def test_turned_keys_do_not_depend_on_how_the_tokens_arrive(lane, pieces):
         got, whole = stored(pieces), stored([sum(pieces)])
         assert np.array_equal(got, whole) and abs(got[0] / (1.2270393371582031 * np.cos(6412 * np.float64(np.float32(0.9)))) - 1) < 2.0 ** -22
     freq.dispose()
+
+
+def test_refusals_of_launches_of_too_many_threads(lane):
+    """A launch holds fewer than 2^32 threads: what would need more is refused before it is tried (8: too large)."""
+    import ctypes
+    from nntrain_amd import native
+    lib, h = lane._lib, lane._handle
+    with QuantizedKvCache(lane, 1, 1, 1, 1, 100) as cache:
+        lane.write(cache.lengths, np.array([-1], np.int32))             # (left out, whatever is asked for)
+        one = lane.allocate(4)
+        still = native.RowsDesc(one.ptr, 0, 0)
+        launches = lane.counters()["kernel_launches"]
+        store = native.KvStoreDesc(struct_size=ctypes.sizeof(native.KvStoreDesc), tokens=2**30, k=still, v=still)
+        assert lib.nnhip_kv_cache_store(h, cache._refs[0], ctypes.byref(store)) == 8
+        far = native.RowsDesc(one.ptr, 1, 2**30)
+        assert lib.nnhip_kv_cache_read(h, cache._refs[0], None, 2**30, ctypes.byref(far), None) == 8
+        many = native.KvCacheDesc(ctypes.sizeof(native.KvCacheDesc), 2**22, 1, 1, 100, 0, one.ptr, cache.lengths.ptr)
+        attend = native.AttentionDesc(struct_size=ctypes.sizeof(native.AttentionDesc), tokens=200, q=still, out=native.RowsDesc(one.ptr + 4, 1, 200),
+                                      heads=1, scale=1.0)
+        assert lib.nnhip_cached_attention(h, ctypes.byref(many), ctypes.byref(attend)) == 8
+        assert lane.counters()["kernel_launches"] == launches
+        one.dispose()
