@@ -472,6 +472,8 @@ class QuantizedDecoder:
         self._room(len(ids))
         d, lane = self.descriptor, self.lane
         log_probs, entropies = [], []
+        if min(rows, len(ids)) > 65535:
+            raise ValueError("rows must be at most 65535.")             # (what one call of token_log_probs takes)
         batch = max(rows, 128 // rows * rows)
         for at in range(0, len(ids), batch):
             part, targets = ids[at:at + batch], ids[at + 1:at + 1 + batch]

@@ -265,3 +265,13 @@ def test_an_architecture_that_turns_halves_of_a_head(lane, tmp_path, monkeypatch
         cpu = CpuContext(host)
         for t in tokens:
             assert oracle.rel_l2(lane.read(dec.forward_token(t), count=VOCAB), cpu.step([t])[0]) <= BAR
+
+
+def test_scores_of_more_rows_than_a_call_takes_are_refused_before_any_work(lane, tmp_path):
+    path, _ = _model(tmp_path, "w.gguf")
+    with _decoder(lane, path, context_length=66000) as dec:
+        launches = lane.counters()["kernel_launches"]
+        with pytest.raises(ValueError):
+            dec.score([1] * 65540, rows=65537)
+        assert dec.position == 0 and lane.counters()["kernel_launches"] == launches
+        assert dec.score([1, 2, 3], rows=65537)[0].shape == (2,)
