@@ -6,7 +6,7 @@
 // and o / l at the end.  All in powers of two: the factor log2(e) goes into the scale.
 //
 // The query rows that share a key/value head (tokens x heads of the group) are the columns of the matrix products, so a block
-// of keys is read once for all of them: S^T = K Q^T, O^T = V^T P^T, on v_mfma_f32_16x16x32_f16 with 16 rows a column tile.
+// of keys is read once for a tile of them: S^T = K Q^T, O^T = V^T P^T, on v_mfma_f32_16x16x32_f16 with 16 rows a column tile.
 // Transposed this way a lane's accumulators hold 16 probabilities of one row, in the order in which the cache keeps the
 // values' tokens (kv_cache_layout.h): they are the operand of the second product as they stand, and a row's maximum needs two
 // exchanges between lanes.
@@ -16,8 +16,11 @@
 // the value scales of the blocks a row has seen) times 2^14: 22 bits below the largest, nothing lost before 2^-38 of it.  Two products for each operand pair
 // instead of one is what FP32 results cost; one rounding to half precision would leave 2^-12.
 //
-// Two kernels.  attend_few_kernel, up to 32 rows a key/value head (decode): bound by reading the cache, so every wave walks over
-// blocks of its own, codes go from memory to registers to half precision without LDS, and the keys are split over many
+// All sums are FP32 and grow a block at a time: l and o of a row over n keys that one workgroup takes are off by up to (n / 16) 2^-23
+// of themselves, seen where one key stands far above many (131000 keys, one 17 above the others, unsplit: 1.1e-4).
+//
+// Two kernels.  attend_few_kernel, up to 32 rows a key/value head (decode): bound by reading the cache, once for 32 rows of heads up
+// to 128 and once for 16 of larger ones, so every wave walks over blocks of its own, codes go from memory to registers to half precision without LDS, and the keys are split over many
 // workgroups.  attend_many_kernel (prompts): bound by the matrix cores and the softmax beside them, so the waves of a tile share
 // each block, converted once into LDS; its keys are split where there are few tiles.  The parts are added up by
 // attend_join_few_kernel (up to eight) or attend_join_kernel.
@@ -329,7 +332,7 @@ __device__ void refuse_rows(const AttendArgs& a, const Span& s, int b, int kv_he
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-// Codes that one workgroup alone reads: streamed past the caches.
+// Codes that one workgroup alone reads (two, where 17 to 32 rows of heads above 128 are two tiles): streamed past the caches.
 __device__ __forceinline__ uint4 stream(const uint8_t* p)
 {
     const u32x4 x = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p));

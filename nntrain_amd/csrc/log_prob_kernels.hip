@@ -567,7 +567,7 @@ LogProbPlan plan_token_log_probs(const nnhip_log_probs_desc& d, int compute_unit
     // 2100 rows of 5000 would take 81 us instead of 25.
     const bool one = pieces <= (d.top > kWaves ? 32 : 16) && d.rows <= compute_units;
     p.waves = one && pieces > kWaves ? 16 : kWaves;
-    // Otherwise eight workgroups of four waves a compute unit, none with less than a piece for each wave.
+    // Otherwise eight workgroups of four waves a compute unit (of which five fit at a time), none with less than a piece for each wave.
     int64_t segments = one ? 1 : 8 * static_cast<int64_t>(compute_units) / d.rows;
     if (segments > (pieces + kWaves - 1) / kWaves) segments = (pieces + kWaves - 1) / kWaves;
     if (segments < 1) segments = 1;

@@ -149,7 +149,8 @@ class QuantizedKvCache:
                   out: "HipBuffer | Rows | None" = None) -> "HipBuffer | Rows":
         """Causal attention of the tokens just stored over the cache: token i of sequence b stands at position lengths[b] + i
         and sees the keys up to it, with window > 0 the last `window` of them and the first `sinks` tokens.  scale: 1 /
-        sqrt(head_width) by default.  FP32 in and out; rows behind counts[b] are left as they are."""
+        sqrt(head_width) by default.  FP32 in and out; rows behind counts[b] are left as they are.  The scale of a block covers
+        all its stored tokens: of tokens stored together, those behind a row have that influence on it."""
         cache = self._cache(layer)
         if not 1 <= tokens <= _LARGEST or not 1 <= heads <= _LARGEST or heads % self.kv_heads != 0:
             raise ValueError("tokens must be positive, heads a positive multiple of kv_heads, both fit 32 bits.")

@@ -780,3 +780,60 @@ def test_refusals_of_launches_of_too_many_threads(lane):
         assert lib.nnhip_cached_attention(h, ctypes.byref(many), ctypes.byref(attend)) == 8
         assert lane.counters()["kernel_launches"] == launches
         one.dispose()
+
+
+def test_tokens_behind_a_row_act_through_the_scale_of_its_block_alone(lane):
+    """A call stores its tokens before it attends: a row reads what the cache then stands for, later tokens in the scale."""
+    kv, heads, width, n = 1, 2, 64, 10
+    rng = _rng(16)
+    k, v, q = _values(rng, n, kv, width), _values(rng, n, kv, width), _values(rng, n, heads, width)
+    for size in (30.0, 1000.0, np.inf):
+        late_k, late_v = k.copy(), v.copy()
+        late_k[n - 1], late_v[n - 1] = size, size
+        with QuantizedKvCache(lane, 1, 1, kv, width, n) as cache:
+            _put(lane, cache, 0, late_k[None], late_v[None])
+            qb = lane.upload_raw(q)
+            out = cache.attention(0, qb, heads, n)
+            together = lane.read(out).reshape(n, heads, width)
+            kq, vq = ref.cached(late_k), ref.cached(late_v)
+            if np.isfinite(size):
+                want, reach = ref.attend(q, kq, vq, 0)
+                assert np.abs(together - want)[:n - 1].max() <= _tolerance(reach, n, width, np.abs(vq[:n - 1]).max() + np.abs(vq).max() / 127)
+            else:
+                assert np.isnan(together).all()
+            # token by token nothing behind a row has any influence
+            cache.reset()
+            for i in range(n - 1):
+                _put(lane, cache, 0, late_k[None, i:i + 1], late_v[None, i:i + 1])
+                part = Rows(qb, heads * width, 0, i * heads * width)
+                one = cache.attention(0, part, heads)
+                want, reach = ref.attend(q[i:i + 1], ref.cached(k[:i + 1]), ref.cached(v[:i + 1]), i)
+                assert np.abs(lane.read(one).reshape(1, heads, width) - want).max() <= _tolerance(reach, i + 1, width, np.abs(v[:i + 1]).max())
+                cache.advance(1)
+                one.dispose()
+            for b in (qb, out):
+                b.dispose()
+
+
+@pytest.mark.parametrize("n", [1, 50, 1100])
+def test_a_tail_far_below_one_key_over_a_long_cache(lane, n):
+    """One key 17 or 21.6 above 30000 others: what a block adds is a few or less than one of the large sum's last places.  Bar:
+    (n / 16) 2^-23 of the sums, numerator and denominator, and the parts of a probability."""
+    width, heads, before = 64, 8, 30000
+    for gap in (17.0, 21.6):
+        k, v = (np.zeros((before + n, heads, width), np.float32) for _ in range(2))
+        k[0, :, 0], v[1:, :, 1], v[0, :, 0] = gap, 1.0, 1.0
+        q = np.zeros((n, heads, width), np.float32)
+        q[..., 0] = 1.0
+        with QuantizedKvCache(lane, 1, 1, heads, width, before + n) as cache:
+            _put(lane, cache, 0, k[None], v[None])
+            cache.set_lengths([before])
+            qb = lane.upload_raw(q)
+            out = cache.attention(0, qb, heads, n, scale=1.0)
+            got = lane.read(out).reshape(n, heads, width)
+            for b in (qb, out):
+                b.dispose()
+        others = ((before + np.arange(n)) * np.exp(-float(np.float32(gap / 127) * np.float32(127))))[:, None]
+        bar = 2 * ((before + n) / 16 * 2.0 ** -23 + 2.0 ** -21)
+        assert np.abs(got[..., 1] - others / (1 + others)).max() <= bar and np.abs(got[..., 0] - 1 / (1 + others)).max() <= bar
+        assert not got[..., 2:].any()
